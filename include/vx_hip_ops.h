@@ -75,6 +75,132 @@ int32_t vx_nn_gemv_i8_bf16(const int8_t *w, const float *scale,
                            const uint16_t *x, float *y, int64_t rows,
                            int64_t cols, int64_t batch);
 
+/* ---- Many answers to one prompt ----------------------------------------
+ *
+ * A step of a batch of sequences that begin with the same prompt: the prompt's
+ * keys and values are stored once, each sequence has a cache of its own for
+ * what follows. vx_nn_rope_append_* turns a fused projection into rotated
+ * queries and new cache rows, vx_nn_flash_attention_shared_bf16 attends over
+ * the shared prefix and the own cache, and vx_nn_sample_* draws the next
+ * tokens from the classifier's logits. No counterpart in the reference.
+ *
+ * lens (device memory, int32 [batch]) says how many rows of its own cache each
+ * sequence has, the step's seq_q new ones among them: query i of sequence b is
+ * at position shared_len + lens[b] - seq_q + i. It is read when the kernels
+ * run, so a captured graph follows it. lens NULL: capacity for all. A slot
+ * whose lens[b] is negative or above capacity holds no sequence: nothing of it
+ * is read, and its outputs and cache stay as they were.
+ *
+ * Arguments are checked before the GPU is looked for, so a refusal is the same
+ * without one. Every pointer must be memory of one GPU; the ops run on that
+ * GPU, whichever is current.
+ *
+ * `workspace`: GPU memory for partial results, 16-byte aligned, its contents
+ * of no account before and after. The calls work with NULL: then the library
+ * keeps a block per (device, stream), taken and freed as attention's split
+ * workspaces are, and a stream that is capturing a graph, or hipStreamPerThread,
+ * gets a launch that needs none. A captured call that shall divide its work
+ * is given one of at least *_workspace() bytes (a smaller one is refused),
+ * which two launches that may run at the same time must not share. */
+
+/* Splits, rotates and appends. qkv: [batch, seq_q, heads + 2 * kv_heads,
+ * head_dim] (a token's queries, keys and values together, as one projection
+ * leaves them), bf16 or f32. rope: [rope_len, head_dim / 2, 2] f32 of (cos,
+ * sin), at least shared_len + capacity rows; NULL: no rotation. q: [batch,
+ * heads, seq_q, head_dim] bf16; k_cache, v_cache: [batch, kv_heads, capacity,
+ * head_dim] bf16.
+ * With at = lens[b] - seq_q + i, the query and key of token i turn by row
+ * shared_len + at of the table, pairs (2 j, 2 j + 1), in f32, rounded to bf16
+ * once; q gets the query, row `at` of the caches the key and value. A token
+ * whose `at` is below 0 belongs to the shared prefix: its query is turned
+ * alike (zeros if it lies before the prefix's begin), its key and value are
+ * not stored. head_dim a multiple of 8, at most 512; pointers 16-byte
+ * aligned; outputs must not overlap qkv. */
+int32_t vx_nn_rope_append_bf16(const uint16_t *qkv, const float *rope,
+                               const int32_t *lens, uint16_t *q,
+                               uint16_t *k_cache, uint16_t *v_cache,
+                               int64_t batch, int64_t seq_q, int64_t heads,
+                               int64_t kv_heads, int64_t head_dim,
+                               int64_t shared_len, int64_t capacity,
+                               int64_t rope_len);
+int32_t vx_nn_rope_append_f32(const float *qkv, const float *rope,
+                              const int32_t *lens, uint16_t *q,
+                              uint16_t *k_cache, uint16_t *v_cache,
+                              int64_t batch, int64_t seq_q, int64_t heads,
+                              int64_t kv_heads, int64_t head_dim,
+                              int64_t shared_len, int64_t capacity,
+                              int64_t rope_len);
+
+/* Attention over a shared prefix and own caches: what
+ * vx_nn_flash_attention_fwd_bf16 computes for each sequence over the shared
+ * keys followed by its own, with the shared keys read for many sequences at
+ * once.
+ * q: [batch, heads, seq_q, head_dim] bf16; k_shared, v_shared: the first
+ * shared_len rows of [kv_heads, shared_capacity, head_dim] bf16; k, v:
+ * [batch, kv_heads, capacity, head_dim] bf16, of which lens[b] rows count
+ * (what the others hold is never looked at); o: like q; lse: [batch, heads,
+ * seq_q] f32 (may be NULL). With `causal`, query i of sequence b sees key j
+ * of shared ++ own iff j <= shared_len + lens[b] - seq_q + i; else all
+ * shared_len + lens[b]. A key that a query does not see does not reach its
+ * result, whatever its values; a query that sees none gets o = 0 and lse =
+ * -inf. k_shared and v_shared may be NULL where shared_len is 0, k and v
+ * where capacity is 0. head_dim 64 or 128; pointers 16-byte aligned. */
+int32_t vx_nn_flash_attention_shared_bf16(
+    const uint16_t *q, const uint16_t *k_shared, const uint16_t *v_shared,
+    const uint16_t *k, const uint16_t *v, const int32_t *lens, uint16_t *o,
+    float *lse, int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
+    int64_t shared_len, int64_t shared_capacity, int64_t capacity,
+    int64_t head_dim, float scale, int32_t causal, void *workspace,
+    int64_t workspace_bytes);
+/* Bytes of workspace that such a call uses (0: none); a negative VX_OP_E*
+ * code for extents it does not take. */
+int64_t vx_nn_flash_attention_shared_workspace(int64_t batch, int64_t heads,
+                                               int64_t kv_heads, int64_t seq_q,
+                                               int64_t shared_len,
+                                               int64_t capacity,
+                                               int64_t head_dim);
+
+/* Next tokens from logits: temperature, top-k, top-p, min-p and one given
+ * uniform number a row.
+ * logits: [rows, vocab] f32 or bf16, rows `stride` elements apart (at least
+ * vocab); u: [rows] f32 in [0, 1); tokens: [rows] int32; logprob: [rows] f32
+ * (may be NULL). The settings are arrays of a value per row, each of which may
+ * be NULL: temperature (1), top_k (off), top_p (off), min_p (off).
+ * With t = logit / temperature and w = exp(t - max t), tokens go in the order
+ * of falling logits, the lower index first among equals. Of that order the
+ * first token stays, and of the others those that every setting keeps:
+ *   top_k: the first top_k (0 or less: all);
+ *   top_p: those before which, of the tokens that top_k keeps, lies less than
+ *     top_p of their weight (1 or more, or NaN: all);
+ *   min_p: those with w >= min_p (0 or less, or NaN: all).
+ * The row's token is the lowest index i of a kept token at which the sum of
+ * the kept weights up to i exceeds u times their sum; logprob is the natural
+ * logarithm of its share of that sum. temperature 0, negative or NaN: the
+ * first token of the order. u outside [0, 1) counts as the nearest number
+ * inside, NaN as 0.
+ * A NaN logit counts as -inf, and what is -inf is never drawn; where a logit
+ * is +inf, those are the only ones, with equal weights. A row without a logit
+ * above -inf gets token -1 and logprob -inf.
+ * Weights are 64-bit integers in units of at most 2^-32 of the row's largest
+ * one (2^-45 at a vocabulary of 131072), so sums are exact and a result does
+ * not depend on how the work is divided; a token whose weight rounds to 0 is
+ * not drawn. vocab at most 2^30. */
+int32_t vx_nn_sample_f32(const float *logits, const float *temperature,
+                         const int32_t *top_k, const float *top_p,
+                         const float *min_p, const float *u, int32_t *tokens,
+                         float *logprob, int64_t rows, int64_t vocab,
+                         int64_t stride, void *workspace,
+                         int64_t workspace_bytes);
+int32_t vx_nn_sample_bf16(const uint16_t *logits, const float *temperature,
+                          const int32_t *top_k, const float *top_p,
+                          const float *min_p, const float *u, int32_t *tokens,
+                          float *logprob, int64_t rows, int64_t vocab,
+                          int64_t stride, void *workspace,
+                          int64_t workspace_bytes);
+/* Bytes of workspace that such a call uses (0: none); VX_OP_EINVAL for
+ * extents it does not take. */
+int64_t vx_nn_sample_workspace(int64_t rows, int64_t vocab);
+
 /* Greedy int8 decode of a Llama-2-style model, resident in HBM.
  *
  * The token step of reference examples/llama.vx:173-420 (RMSNorm eps 1e-5,

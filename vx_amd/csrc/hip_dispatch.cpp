@@ -141,17 +141,20 @@ void select_device(int32_t topology_id, const char *why) {
 
 /* True for memory the GPU owns (hipMalloc'd). Host memory, registered or not,
  * answers false. */
-bool is_device_ptr(const void *p) {
+/* The GPU whose memory `p` is, -1 where it is not GPU memory. */
+int device_of_ptr(const void *p) {
   if (!p || !hip_available()) {
-    return false;
+    return -1;
   }
   hipPointerAttribute_t attr;
   if (hipPointerGetAttributes(&attr, p) != hipSuccess) {
     (void)hipGetLastError();
-    return false;
+    return -1;
   }
-  return attr.type == hipMemoryTypeDevice;
+  return attr.type == hipMemoryTypeDevice ? attr.device : -1;
 }
+
+bool is_device_ptr(const void *p) { return device_of_ptr(p) >= 0; }
 
 void *device_malloc(size_t bytes) {
   void *p = nullptr;
@@ -1010,6 +1013,7 @@ namespace vxops {
 hipStream_t stream() { return caller_stream; }
 bool device_present() { return hip_available(); }
 bool on_device(const void *p) { return is_device_ptr(p); }
+int device_of(const void *p) { return device_of_ptr(p); }
 void launched(const char *what) { started_kernel(what); }
 bool chatty() { return verbose(); }
 bool capturing() { return ::capturing(); }

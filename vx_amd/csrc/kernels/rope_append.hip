@@ -1,0 +1,114 @@
+/*
+ * rope_append.hip -- a fused projection split into rotated queries and new
+ * rows of each sequence's cache (vx_nn_rope_append_*).
+ *
+ * (x0, x1) -> (x0 c - x1 s, x0 s + x1 c) for the pairs of a head, in f32,
+ * rounded to bf16 once. Bound by memory: each element of the projection is
+ * read once and written once, the table's rows come from L2 after their first
+ * head. A thread takes 8 elements, 16 bytes of output and 32 of the table.
+ */
+#include "../vx_batch_kernels.h"
+#include "../vx_hip_common.h"
+
+namespace vxk {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kThreads = 256;
+
+template <bool kF32> __device__ __forceinline__ void load8(const void *p, int64_t at, float (&x)[8]) {
+  if constexpr (kF32) {
+    const f32x4 *src = reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + at);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 v = src[h];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[4 * h + e] = v[e];
+      }
+    }
+  } else {
+    const u32x4 v = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(p) + at);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[2 * e] = __uint_as_float(v[e] << 16);
+      x[2 * e + 1] = __uint_as_float(v[e] & 0xffff0000u);
+    }
+  }
+}
+
+template <bool kF32>
+__global__ __launch_bounds__(kThreads) void rope_append(RopeAppendArgs a, int64_t units) {
+  const int64_t unit = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (unit >= units) {
+    return;
+  }
+  const int per_head = a.head_dim / 8;
+  const int all = a.heads + 2 * a.kv_heads;
+  const int c = (int)(unit % per_head) * 8;
+  const int64_t row = unit / per_head; /* of head_dim elements */
+  const int h = (int)(row % all);
+  const int64_t token = row / all;
+  const int i = (int)(token % a.seq_q);
+  const int64_t b = token / a.seq_q;
+  const int64_t len = a.lens ? a.lens[b] : a.capacity;
+  if (len < 0 || len > a.capacity) {
+    return;
+  }
+  const int64_t at = len - a.seq_q + i;
+  const int64_t pos = a.shared_len + at;
+  const bool query = h < a.heads;
+  if (!query && at < 0) {
+    return;
+  }
+  float x[8];
+  load8<kF32>(a.qkv, row * a.head_dim + c, x);
+  if (pos < 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[e] = 0.0f;
+    }
+  } else if (a.rope && h < a.heads + a.kv_heads) {
+    float t[8];
+    load8<true>(a.rope, pos * a.head_dim + c, t);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float x0 = x[e], x1 = x[e + 1];
+      x[e] = x0 * t[e] - x1 * t[e + 1];
+      x[e + 1] = x0 * t[e + 1] + x1 * t[e];
+    }
+  }
+  uint16_t *dst;
+  if (query) {
+    dst = a.q + ((b * a.heads + h) * a.seq_q + i) * a.head_dim + c;
+  } else {
+    const int kv = h - a.heads;
+    const bool key = kv < a.kv_heads;
+    dst = (key ? a.k_cache : a.v_cache) +
+          ((b * a.kv_heads + (key ? kv : kv - a.kv_heads)) * a.capacity + at) * a.head_dim + c;
+  }
+  u32x4 out;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    out[e] = (uint32_t)f32_to_bf16(x[2 * e]) | (uint32_t)f32_to_bf16(x[2 * e + 1]) << 16;
+  }
+  *reinterpret_cast<u32x4 *>(dst) = out;
+}
+
+} // namespace
+
+void rope_append_launch(const RopeAppendArgs &a, hipStream_t stream) {
+  const int64_t units =
+      a.batch * a.seq_q * (a.heads + 2 * (int64_t)a.kv_heads) * (a.head_dim / 8);
+  const dim3 grid((unsigned)((units + kThreads - 1) / kThreads));
+  if (a.f32) {
+    hipLaunchKernelGGL((rope_append<true>), grid, dim3(kThreads), 0, stream, a, units);
+  } else {
+    hipLaunchKernelGGL((rope_append<false>), grid, dim3(kThreads), 0, stream, a, units);
+  }
+  VX_HIP_CHECK(hipGetLastError());
+}
+
+} // namespace vxk

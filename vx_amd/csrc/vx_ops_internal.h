@@ -12,6 +12,8 @@ namespace vxops {
 hipStream_t stream();
 bool device_present();
 bool on_device(const void *p);
+/* The GPU whose memory `p` is, -1 where it is not GPU memory. */
+int device_of(const void *p);
 void launched(const char *what);
 bool chatty();
 /* Whether the caller stream is capturing a hipGraph now. */

@@ -64,6 +64,14 @@ HIP_SIGNATURES = {
     "vx_nn_flash_attention_fwd_bf16": (
         _i32, [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, ctypes.c_float, _i32]),
     "vx_nn_gemv_i8_bf16": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _i64]),
+    "vx_nn_rope_append_bf16": (_i32, [_vp] * 6 + [_i64] * 8),
+    "vx_nn_rope_append_f32": (_i32, [_vp] * 6 + [_i64] * 8),
+    "vx_nn_flash_attention_shared_bf16": (
+        _i32, [_vp] * 8 + [_i64] * 8 + [ctypes.c_float, _i32, _vp, _i64]),
+    "vx_nn_flash_attention_shared_workspace": (_i64, [_i64] * 7),
+    "vx_nn_sample_f32": (_i32, [_vp] * 8 + [_i64] * 3 + [_vp, _i64]),
+    "vx_nn_sample_bf16": (_i32, [_vp] * 8 + [_i64] * 3 + [_vp, _i64]),
+    "vx_nn_sample_workspace": (_i64, [_i64, _i64]),
     "vx_llama_i8_create": (_vp, [_vp, _vp, _u32]),
     "vx_llama_i8_generate": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _i32]),
     "vx_llama_i8_logits": (_i32, [_vp, _vp, _i32, _vp]),
@@ -264,6 +272,39 @@ def flash_attention_fwd(lib: DispatchLibrary, q: int, k: int, v: int, o: int, ls
 def gemv_i8(lib: DispatchLibrary, w: int, scale: int, x: int, y: int, rows: int, cols: int,
             batch: int) -> int:
     return lib.lib.vx_nn_gemv_i8_bf16(w, scale, x, y, rows, cols, batch)
+
+
+def rope_append(lib: DispatchLibrary, dtype: str, qkv: int, rope: int | None, lens: int | None,
+                q: int, k_cache: int, v_cache: int, batch: int, seq_q: int, heads: int,
+                kv_heads: int, head_dim: int, shared_len: int, capacity: int,
+                rope_len: int) -> int:
+    """vx_nn_rope_append_<dtype> ("bf16" or "f32": the projection's type)."""
+    fn = {"bf16": lib.lib.vx_nn_rope_append_bf16, "f32": lib.lib.vx_nn_rope_append_f32}[dtype]
+    return fn(qkv, rope, lens, q, k_cache, v_cache, batch, seq_q, heads, kv_heads, head_dim,
+              shared_len, capacity, rope_len)
+
+
+def flash_attention_shared(lib: DispatchLibrary, q: int, k_shared: int | None,
+                           v_shared: int | None, k: int | None, v: int | None, lens: int | None,
+                           o: int, lse: int | None, batch: int, heads: int, kv_heads: int,
+                           seq_q: int, shared_len: int, capacity: int, head_dim: int,
+                           scale: float, causal: bool, shared_capacity: int | None = None,
+                           workspace: int | None = None, workspace_bytes: int = 0) -> int:
+    """vx_nn_flash_attention_shared_bf16; shared_capacity None: shared_len."""
+    return lib.lib.vx_nn_flash_attention_shared_bf16(
+        q, k_shared, v_shared, k, v, lens, o, lse, batch, heads, kv_heads, seq_q, shared_len,
+        shared_len if shared_capacity is None else shared_capacity, capacity, head_dim, scale,
+        1 if causal else 0, workspace, workspace_bytes)
+
+
+def sample(lib: DispatchLibrary, dtype: str, logits: int, temperature: int | None,
+           top_k: int | None, top_p: int | None, min_p: int | None, u: int, tokens: int,
+           logprob: int | None, rows: int, vocab: int, stride: int | None = None,
+           workspace: int | None = None, workspace_bytes: int = 0) -> int:
+    """vx_nn_sample_<dtype> ("f32" or "bf16": the logits' type); stride None: vocab."""
+    fn = {"f32": lib.lib.vx_nn_sample_f32, "bf16": lib.lib.vx_nn_sample_bf16}[dtype]
+    return fn(logits, temperature, top_k, top_p, min_p, u, tokens, logprob, rows, vocab,
+              vocab if stride is None else stride, workspace, workspace_bytes)
 
 
 class HipTimer:
