@@ -48,6 +48,7 @@ HIP_CTRL_FA_SPLITS = CTRL_VENDOR_BASE + 7
 HIP_CTRL_FA_WORKSPACES = CTRL_VENDOR_BASE + 8
 HIP_CTRL_STAGING_STATS = CTRL_VENDOR_BASE + 9
 HIP_CTRL_GEMM_WORKSPACES = CTRL_VENDOR_BASE + 10
+HIP_CTRL_OP_WORKSPACES = CTRL_VENDOR_BASE + 11
 # Kernels the GEMV control opcode can force (0 = automatic choice).
 GEMV_AUTO, GEMV_ROWS, GEMV_DOT2_B4, GEMV_LDS = 0, 1, 2, 3
 # Kernels the GEMM control opcode can force (0 = automatic choice).

@@ -41,6 +41,7 @@
  */
 #include "../../include/vx_hardware_runtime.h"
 #include "../../include/vx_hip_ops.h"
+#include "op_space.h"
 #include "vx_device_pool_hip.h"
 #include "vx_dispatch_plan.h"
 #include "vx_hip_common.h"
@@ -1343,6 +1344,7 @@ int32_t vx_hip_image_param_count(const void *image, size_t image_size,
 #define VX_HIP_CTRL_FA_WORKSPACES (VX_CTRL_VENDOR_BASE + 8)
 #define VX_HIP_CTRL_STAGING_STATS (VX_CTRL_VENDOR_BASE + 9)
 #define VX_HIP_CTRL_GEMM_WORKSPACES (VX_CTRL_VENDOR_BASE + 10)
+#define VX_HIP_CTRL_OP_WORKSPACES (VX_CTRL_VENDOR_BASE + 11)
 
 int32_t vx_plugin_control(uint32_t opcode, void *payload) {
   switch (opcode) {
@@ -1514,6 +1516,16 @@ int32_t vx_plugin_control(uint32_t opcode, void *payload) {
     out[3] = vxk::device_cu_count();
     return 1;
   }
+  case VX_HIP_CTRL_OP_WORKSPACES: {
+    /* payload -> int64_t[2]: workspaces held for the ops of a batch that
+     * shares a prompt (one per device and stream) and their bytes. */
+    int64_t *out = static_cast<int64_t *>(payload);
+    if (!out) {
+      return 0;
+    }
+    vxk::op_space_stats(&out[0], &out[1]);
+    return 1;
+  }
   case VX_HIP_CTRL_POOL_DRAIN:
     if (hip_available()) {
       wait_for_kernels("pool drain");
@@ -1550,6 +1562,7 @@ void vx_hip_set_stream(void *stream) {
   if (caller_stream && caller_stream != next) {
     vxk::flash_attn_release_stream(caller_stream);
     vxk::gemm_release_stream(caller_stream);
+    vxk::op_space_release_stream(caller_stream);
   }
   caller_stream = next;
 }

@@ -7,6 +7,7 @@
  * the one the kernels run on whichever is current.
  */
 #include "../../include/vx_hip_ops.h"
+#include "op_space.h"
 #include "vx_batch_kernels.h"
 #include "vx_hip_common.h"
 #include "vx_ops_internal.h"
@@ -91,6 +92,29 @@ public:
 private:
   int before_ = 0;
   bool moved_ = false;
+};
+
+/* A launch's workspace: the caller's, or the one kept for the stream, held
+ * through the scope. A stream that is capturing a graph, or a handle of
+ * several streams, has none of the library's. */
+class Space {
+public:
+  Space(void *given, int64_t bytes) {
+    if (bytes == 0 || given) {
+      base = static_cast<char *>(given);
+      enough = true;
+    } else if (vxk::one_stream(vxops::stream()) && !vxops::capturing()) {
+      hold_ = vxk::op_space_lock();
+      base = vxk::op_space((size_t)bytes, vxops::stream());
+      enough = base != nullptr;
+    }
+  }
+
+  char *base = nullptr;
+  bool enough = false;
+
+private:
+  std::unique_lock<std::mutex> hold_;
 };
 
 /* The product of extents that are each at most 2^40, or -1 past 2^62. */
@@ -234,7 +258,12 @@ int64_t vx_nn_flash_attention_shared_workspace(int64_t batch, int64_t heads, int
   const char *why = nullptr;
   const int32_t code = shared_extents(batch, heads, kv_heads, seq_q, shared_len, capacity,
                                       head_dim, &why);
-  return code == VX_OP_OK ? 0 : code;
+  if (code != VX_OP_OK) {
+    return code;
+  }
+  return vxk::flash_shared_plan(batch, (int)heads, (int)kv_heads, (int)seq_q, (int)shared_len,
+                                (int)capacity, (int)head_dim, vxk::device_cu_count(), true)
+      .ws_bytes;
 }
 
 int32_t vx_nn_flash_attention_shared_bf16(
@@ -275,11 +304,16 @@ int32_t vx_nn_flash_attention_shared_bf16(
   if (on.code != VX_OP_OK) {
     return on.code;
   }
-  vxk::flash_shared_launch(
-      vxk::SharedAttnArgs{q, k_shared, v_shared, k, v, lens, o, lse, (int)batch, (int)heads,
-                          (int)kv_heads, (int)seq_q, (int)shared_len, shared_capacity,
-                          (int)capacity, scale, causal != 0},
-      (int)head_dim, vxops::stream());
+  const vxk::SharedAttnArgs args{q, k_shared, v_shared, k, v, lens, o, lse, (int)batch,
+                                 (int)heads, (int)kv_heads, (int)seq_q, (int)shared_len,
+                                 shared_capacity, (int)capacity, scale, causal != 0};
+  auto plan = [&](bool may_split) {
+    return vxk::flash_shared_plan(batch, (int)heads, (int)kv_heads, (int)seq_q, (int)shared_len,
+                                  (int)capacity, (int)head_dim, vxk::device_cu_count(),
+                                  may_split);
+  };
+  const Space space(workspace, plan(true).ws_bytes);
+  vxk::flash_shared_launch(args, plan(space.enough), (int)head_dim, space.base, vxops::stream());
   vxops::launched(op);
   return VX_OP_OK;
 }
