@@ -128,6 +128,14 @@ __device__ __forceinline__ uint32_t not_finite(uint32_t w) {
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
+/* The lane's number, read again: an address made from it where it is used needs
+ * no register in between. */
+__device__ __forceinline__ int lane_here() {
+  int v;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(v));
+  return v;
+}
+
 __device__ __forceinline__ int wave_min(int v) {
   for (int o = 32; o; o >>= 1) {
     v = min(v, __shfl_xor(v, o));
@@ -179,7 +187,12 @@ template <int kChunks> __device__ __forceinline__ int place_v(int key, int c) {
   }
 }
 
-template <int kD> constexpr int wide_lds() { return 4 * kBK * kD * 2; }
+/* The last d-step of a query waits in LDS where its registers would be spilled
+ * (to memory, whose reload waits for the keys in flight). */
+template <int kD, int kGroups> constexpr bool kParkQ = kD == 128 && kGroups == 1;
+template <int kD, int kGroups> constexpr int wide_lds() {
+  return 4 * kBK * kD * 2 + (kParkQ<kD, kGroups> ? kThreads * 16 : 0);
+}
 
 /* A tile of 128 / kGroups rows. */
 template <int kD, int kGroups>
@@ -203,7 +216,6 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
   const int g = lane >> 5;
   const int grp = kGroups == 1 ? 0 : wave / kWavesQ;
   const int wq = kGroups == 1 ? wave : wave % kWavesQ;
-  const int tg = kGroups == 1 ? t : t % kGroupThreads;
 
   const Row row = row_of(p, it, 32 * wq + lq);
   const bool real = row.place >= 0;
@@ -231,15 +243,16 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
   for (int s = 0; s < kDSteps; ++s) {
     qf[s] = query(p, row, kD, 8 * g + 16 * s);
   }
-
-  uint32_t k_off[kLoads], v_off[kLoads];
-#pragma unroll
-  for (int l = 0; l < kLoads; ++l) {
-    const int u = l * kGroupThreads + tg;
-    const int key = u / kChunks;
-    k_off[l] = (uint32_t)(key * kRowBytes + place_k<kChunks>(key, u % kChunks) * 16);
-    v_off[l] = (uint32_t)(key * kRowBytes + place_v<kChunks>(key, u % kChunks) * 16);
+  VX_LDS u32x4 *parked = (VX_LDS u32x4 *)(lds + 4 * kBK * kD * 2) + t;
+  if constexpr (kParkQ<kD, kGroups>) {
+    *parked = qf[kDSteps - 1];
   }
+
+  /* Load l of a thread fills unit l * kGroupThreads + tg of a plane: key row
+   * l * kRowsPer + tg / kChunks, whose place differs from l = 0's by an XOR. */
+  constexpr int kRowsPer = kGroupThreads / kChunks;
+  static_assert(kChunks == 16 ? 16 % kRowsPer == 0 && kRowsPer % 4 == 0 : kRowsPer % 16 == 0,
+                "places of the loads of a thread");
   /* [group][slot][K|V][unit] */
   u32x4 *ring = reinterpret_cast<u32x4 *>(lds) + grp * 4 * kUnits;
   const uint32_t ring_base = (uint32_t)(uintptr_t)(VX_LDS void *)ring;
@@ -261,14 +274,35 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
       rs[w] = __builtin_amdgcn_readfirstlane(rs[w]); /* uniform, which the compiler cannot tell */
     }
     const uint32_t base = ring_base + (uint32_t)((((j & 1) * 2 + plane) * kUnits + wq * 64) * 16);
+    const int tg = wq * 64 + lane_here();
+    const int row = tg / kChunks, c = tg % kChunks;
+    const int off =
+        row * kRowBytes + (plane == 0 ? place_k<kChunks>(row, c) : place_v<kChunks>(row, c)) * 16;
 #pragma unroll
     for (int l = 0; l < kLoads; ++l) {
-      dma16(rs, plane == 0 ? k_off[l] : v_off[l], base + (uint32_t)(l * kGroupThreads * 16));
+      const int turn = plane == 0 && kChunks == 16 ? (l * kRowsPer & 15) << 4 : 0;
+      dma16(rs, (uint32_t)((off ^ turn) + l * kRowsPer * kRowBytes),
+            base + (uint32_t)(l * kGroupThreads * 16));
     }
   };
 
-  const int tr_key = 4 * g + ((lane & 15) >> 2);
-  const int tr_d = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+  /* Where the lane reads in a slot's K plane (row lq, chunk g: chunk 2 ds + g
+   * of a place that is an XOR lies at the address XOR 32 ds) and, transposing,
+   * in its V plane: key 4 g + i / 4 of a 16-key step, d 16 j + 4 (i % 4) of a
+   * 32-wide tile, i = lane % 16, j = lane / 16 % 2, which hands it the 8 keys
+   * of its k-slots at d = lane % 32; tile i lies at XOR 64 i. */
+  auto keys_at = [&](int j) {
+    const int l = lane_here();
+    return ring_base + (uint32_t)((j & 1) * 2 * kUnits * 16 + (l & 31) * kRowBytes +
+                                  place_k<kChunks>(l & 31, l >> 5) * 16);
+  };
+  auto values_at = [&](int j) {
+    const int l = lane_here();
+    const int key = 4 * (l >> 5) + ((l & 15) >> 2);
+    const int d = 16 * ((l >> 4) & 1) + 4 * (l & 3);
+    return ring_base + (uint32_t)(((j & 1) * 2 + 1) * kUnits * 16 + key * kRowBytes +
+                                  place_v<kChunks>(key, d >> 3) * 16 + (d & 7) * 2);
+  };
 
   f32x16 o[kDTiles];
 #pragma unroll
@@ -279,14 +313,15 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
 
   typedef f32x16 Scores[kKT];
   auto scores = [&](int j, Scores &st) {
-    const u32x4 *kl = ring + (j & 1) * 2 * kUnits;
+    const uint32_t at = keys_at(j);
 #pragma unroll
     for (int ds = 0; ds < kDSteps; ++ds) {
+      const u32x4 q = kParkQ<kD, kGroups> && ds == kDSteps - 1 ? *parked : qf[ds];
 #pragma unroll
       for (int kt = 0; kt < kKT; ++kt) {
-        const int r = kt * 32 + lq;
-        st[kt] = mfma32(kl[r * kChunks + place_k<kChunks>(r, 2 * ds + g)], qf[ds],
-                        ds == 0 ? f32x16{} : st[kt]);
+        const u32x4 a =
+            *(const VX_LDS u32x4 *)(uintptr_t)((at ^ (uint32_t)(ds << 5)) + (uint32_t)(kt * 32 * kRowBytes));
+        st[kt] = mfma32(a, q, ds == 0 ? f32x16{} : st[kt]);
       }
     }
   };
@@ -334,27 +369,26 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
   };
 
   /* V^T's operand of 16-key step ks and d tile i of turn j. */
-  auto values = [&](int j, int ks, int i) {
-    const VX_LDS char *vl = (const VX_LDS char *)(ring + ((j & 1) * 2 + 1) * kUnits);
-    const int d = 32 * i + tr_d;
+  auto values = [&](uint32_t at, int ks, int i) {
     u32x4 a;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int key = 16 * ks + tr_key + 8 * h;
-      const int at = key * kRowBytes + place_v<kChunks>(key, d >> 3) * 16 + (d & 7) * 2;
       const u32x2 w = __builtin_bit_cast(
-          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((VX_LDS i16x4 *)(vl + at)));
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                     (VX_LDS i16x4 *)(uintptr_t)((at ^ (uint32_t)(i << 6)) +
+                                                 (uint32_t)((16 * ks + 8 * h) * kRowBytes))));
       a[2 * h] = w[0];
       a[2 * h + 1] = w[1];
     }
     return a;
   };
   auto accumulate = [&](int j, const u32x4 (&pt)[kKS]) {
+    const uint32_t at = values_at(j);
 #pragma unroll
     for (int ks = 0; ks < kKS; ++ks) {
 #pragma unroll
       for (int i = 0; i < kDTiles; ++i) {
-        o[i] = mfma32(values(j, ks, i), pt[ks], o[i]);
+        o[i] = mfma32(values(at, ks, i), pt[ks], o[i]);
       }
     }
     /* the transposing reads run ahead of the products that take them */
@@ -370,16 +404,18 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
   /* The same a key at a time, each for the queries that see it: those whose
    * last key of the block, `seen`, is no lower. */
   auto accumulate_apart = [&](int j, const u32x4 (&pt)[kKS], int seen) {
+    const uint32_t at = values_at(j);
+    const int vg = lane_here() >> 5;
 #pragma unroll
     for (int ks = 0; ks < kKS; ++ks) {
 #pragma unroll 1
       for (int n = 0; n < 16; ++n) {
         /* slot e of a lane: key 4 g + e of the step, from e = 4 on 8 more */
         const int e = (n & 3) + 4 * (n >> 3);
-        const uint32_t half = ((n >> 2) & 1) != g ? 0u : e & 1 ? 0xffff0000u : 0xffffu;
+        const uint32_t half = ((n >> 2) & 1) != vg ? 0u : e & 1 ? 0xffff0000u : 0xffffu;
 #pragma unroll
         for (int i = 0; i < kDTiles; ++i) {
-          u32x4 one = values(j, ks, i);
+          u32x4 one = values(at, ks, i);
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
             one[w] &= e >> 1 == w ? half : 0u;
@@ -427,7 +463,7 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
       for (int i = 0; i < kDSteps * kKT; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); /* MFMA */
         __builtin_amdgcn_sched_group_barrier(0x002, 3, 0); /* VALU */
-        if (i < kDSteps * kKT - 4) {
+        if (i < kDSteps * kKT - 4 + (kParkQ<kD, kGroups> ? 1 : 0)) {
           __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
       }
@@ -436,13 +472,14 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
         scores(j + 1, sn);
       }
       if (need_mask) {
-        const int seen = min(limit - base, keys - 1); /* the last key of the block it sees */
+        /* the last key of the block it sees, against constants: keys that are
+         * registers would be kept through the loop, and spilled */
+        const int seen = min(limit - base, keys - 1) - 4 * (lane_here() >> 5);
 #pragma unroll
         for (int kt = 0; kt < kKT; ++kt) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            const int key = 32 * kt + 8 * (r >> 2) + 4 * g + (r & 3);
-            st[kt][r] = key <= seen ? st[kt][r] : -INFINITY;
+            st[kt][r] = 32 * kt + 8 * (r >> 2) + (r & 3) <= seen ? st[kt][r] : -INFINITY;
           }
         }
       }
@@ -459,11 +496,12 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
     }
     if (hidden) {
       uint32_t any = 0;
+      const uint32_t at = values_at(j);
 #pragma unroll 1
       for (int ks = 0; ks < kKS; ++ks) {
 #pragma unroll
         for (int i = 0; i < kDTiles; ++i) {
-          const u32x4 a = values(j, ks, i);
+          const u32x4 a = values(at, ks, i);
           any |= not_finite(a[0]) | not_finite(a[1]) | not_finite(a[2]) | not_finite(a[3]);
         }
       }
@@ -849,9 +887,9 @@ __device__ __forceinline__ void rows16(const KernelArgs &p, const Item &it, char
  * (with plan.together: both). */
 template <int kD, bool kSharedRows, int kGroups, bool kOwnRows>
 __global__ __launch_bounds__(kThreads, 2) void flash_shared(KernelArgs p) {
-  constexpr int kLds = std::max(kSharedRows && kOwnRows ? 0 : wide_lds<kD>(),
+  constexpr int kLds = std::max(kSharedRows && kOwnRows ? 0 : wide_lds<kD, kGroups>(),
                             kSharedRows || kOwnRows ? rows_lds<kD>() : 0);
-  __shared__ __align__(16) char lds[kLds];
+  __shared__ __align__(1024) char lds[kLds]; /* addresses in it are XORed */
   const SharedAttnArgs &a = p.a;
   Item it;
   const int id = blockIdx.x;
