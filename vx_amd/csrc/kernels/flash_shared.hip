@@ -53,8 +53,14 @@ struct KernelArgs {
   uint32_t q_and, q_xor;
   int group, rows_seq; /* heads of a KV head; their queries of one sequence */
   SharedPlan p;
-  char *ws; /* [parts][rows][kD] sums, then [parts][rows][2] max (base 2), weight */
+  char *ws;
 };
+
+/* The workspace's part `part`: [rows][kD] sums, then [rows] statistics (max in
+ * base 2, weight). */
+template <int kD> __device__ __forceinline__ float *part_of(const KernelArgs &p, int part) {
+  return reinterpret_cast<float *>(p.ws) + part * (int64_t)p.p.rows * (kD + 2);
+}
 
 struct Segment {
   const uint16_t *k, *v;
@@ -68,6 +74,7 @@ struct Item {
   int kv, b, row0, part;
   Segment seg[2];
   int blocks0, first, last;
+  int end; /* the last block any query of the tile sees */
 
   __device__ __forceinline__ const uint16_t *k(int s) const { return s ? seg[1].k : seg[0].k; }
   __device__ __forceinline__ const uint16_t *v(int s) const { return s ? seg[1].v : seg[0].v; }
@@ -79,31 +86,28 @@ __device__ __forceinline__ int own_keys(const SharedAttnArgs &a, int b) {
   return n > a.capacity ? -1 : n;
 }
 
-/* Row r of an item's tile: its place among all queries, and the last key it
- * sees, counted from the first shared one; place -1: no such row, or its slot
- * holds no sequence. */
+/* Row r of an item's tile: its place among all queries (-1: past the last),
+ * the last key it sees, counted from the first shared one, and whether its
+ * slot holds a sequence. */
 struct Row {
   int place, limit;
+  bool real;
 };
-__device__ __forceinline__ Row row_of(const KernelArgs &p, const Item &it, int r) {
-  r += it.row0;
-  const int b = it.b >= 0 ? it.b : r / p.rows_seq;
-  const int rem = it.b >= 0 ? r : r - b * p.rows_seq;
+__device__ __forceinline__ Row row_of(const KernelArgs &p, int kv, int b, int r) {
+  const int rem = b >= 0 ? r : r % p.rows_seq;
+  b = b >= 0 ? b : r / p.rows_seq;
   if (b >= p.a.batch || rem >= p.rows_seq) {
-    return Row{-1, -1};
+    return Row{-1, -1, false};
   }
   const int own = own_keys(p.a, b);
-  if (own < 0) {
-    return Row{-1, -1};
-  }
   const int total = p.a.shared_len + own;
   const int i = rem % p.a.seq_q;
-  return Row{(b * p.a.heads + it.kv * p.group) * p.a.seq_q + rem,
-             p.a.causal ? min(total - 1, total - p.a.seq_q + i) : total - 1};
+  return Row{(b * p.a.heads + kv * p.group) * p.a.seq_q + rem,
+             p.a.causal ? min(total - 1, total - p.a.seq_q + i) : total - 1, own >= 0};
 }
 
-/* Eight elements of a row's query, from column c on; zeros where there is no
- * row. The scale's sign goes into the query, so that a hidden key's score is
+/* Eight elements of a row's query, from column c on; of a row that is none they
+ * stay in its own column of every product. The scale's sign goes into the query, so that a hidden key's score is
  * -inf whatever the scale. */
 __device__ __forceinline__ u32x4 query(const KernelArgs &p, const Row &row, int head_dim, int c) {
   u32x4 q = {0, 0, 0, 0};
@@ -151,9 +155,26 @@ __device__ __forceinline__ int wave_max(int v) {
 
 /* The block (of `size` keys) that holds key `limit`; -1 for none. */
 __device__ __forceinline__ int block_of(const Item &it, int limit, int size) {
-  return limit < 0               ? -1
+  return limit == INT32_MAX        ? INT32_MAX
+         : limit < 0               ? -1
          : limit < it.seg[0].keys ? limit / size
                                   : it.blocks0 + (limit - it.seg[0].keys) / size;
+}
+
+/* The least and the greatest limit of the wave's rows; of real ones only, and
+ * INT32_MAX and -1 where there are none. */
+struct Limits {
+  int lo, hi;
+};
+__device__ __forceinline__ Limits limits_of(const KernelArgs &p, const Item &it, const Row &row) {
+  const bool real = row.real;
+  const int all = it.keys(0) + it.keys(1) - 1;
+  /* most often every row sees all of the item's keys */
+  if (__builtin_amdgcn_ballot_w64(real && row.limit < all) == 0) {
+    return Limits{INT32_MAX, __builtin_amdgcn_ballot_w64(real) ? INT32_MAX : -1};
+  }
+  return Limits{__builtin_amdgcn_readfirstlane(wave_min(real ? row.limit : INT32_MAX)),
+                __builtin_amdgcn_readfirstlane(wave_max(real ? row.limit : -1))};
 }
 
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
@@ -217,37 +238,6 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
   const int grp = kGroups == 1 ? 0 : wave / kWavesQ;
   const int wq = kGroups == 1 ? wave : wave % kWavesQ;
 
-  const Row row = row_of(p, it, 32 * wq + lq);
-  const bool real = row.place >= 0;
-  const int lim_lo = __builtin_amdgcn_readfirstlane(wave_min(real ? row.limit : INT32_MAX));
-  const int lim_hi = __builtin_amdgcn_readfirstlane(wave_max(real ? row.limit : -1));
-  const int limit = real ? row.limit : lim_hi;
-  /* The last block any of the wave's queries sees, and any of the tile's. */
-  const int wave_last = min(it.last - 1, block_of(it, lim_hi, kTileKeys));
-  int end = wave_last;
-  {
-    int *ends = reinterpret_cast<int *>(lds);
-    if (lane == 0) {
-      ends[wave] = wave_last;
-    }
-    __syncthreads();
-    end = max(max(ends[0], ends[1]), max(ends[2], ends[3])) + 1;
-    end = __builtin_amdgcn_readfirstlane(end);
-    __syncthreads();
-  }
-  /* Turns: a group's j-th block is first + j * kGroups + grp. */
-  const int turns = end > it.first ? (end - it.first + kGroups - 1) / kGroups : 0;
-
-  u32x4 qf[kDSteps];
-#pragma unroll
-  for (int s = 0; s < kDSteps; ++s) {
-    qf[s] = query(p, row, kD, 8 * g + 16 * s);
-  }
-  VX_LDS u32x4 *parked = (VX_LDS u32x4 *)(lds + 4 * kBK * kD * 2) + t;
-  if constexpr (kParkQ<kD, kGroups>) {
-    *parked = qf[kDSteps - 1];
-  }
-
   /* Load l of a thread fills unit l * kGroupThreads + tg of a plane: key row
    * l * kRowsPer + tg / kChunks, whose place differs from l = 0's by an XOR. */
   constexpr int kRowsPer = kGroupThreads / kChunks;
@@ -285,6 +275,36 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
             base + (uint32_t)(l * kGroupThreads * 16));
     }
   };
+
+  /* Turns: a group's j-th block is first + j * kGroups + grp. The first two of K
+   * and the first of V are on their way before anything else is looked at. */
+  const int end = min(it.last - 1, it.end) + 1;
+  const int turns = end > it.first ? (end - it.first + kGroups - 1) / kGroups : 0;
+  if (turns > 0) {
+    issue(0, 0);
+    issue(0, 1);
+    if (turns > 1) {
+      issue(1, 0);
+    }
+  }
+
+  const Row row = row_of(p, it.kv, it.b, it.row0 + 32 * wq + lq);
+  const bool real = row.real;
+  u32x4 qf[kDSteps];
+#pragma unroll
+  for (int s = 0; s < kDSteps; ++s) {
+    qf[s] = query(p, row, kD, 8 * g + 16 * s);
+  }
+  const Limits lim = limits_of(p, it, row);
+  const int limit = real ? row.limit : lim.hi;
+  const int lim_lo = lim.lo;
+  /* the last block any of the wave's queries sees */
+  const int wave_last = min(end - 1, block_of(it, lim.hi, kTileKeys));
+  VX_LDS u32x4 *parked = (VX_LDS u32x4 *)(lds + 4 * kBK * kD * 2) + t;
+  if constexpr (kParkQ<kD, kGroups>) {
+    *parked = qf[kDSteps - 1];
+  }
+
 
   /* Where the lane reads in a slot's K plane (row lq, chunk g: chunk 2 ds + g
    * of a place that is an XOR lies at the address XOR 32 ds) and, transposing,
@@ -515,11 +535,6 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
 
   Scores sa, sb;
   if (turns > 0) {
-    issue(0, 0);
-    issue(0, 1);
-    if (turns > 1) {
-      issue(1, 0);
-    }
     wait_vm<0>();
     lds_barrier();
     if (it.first + grp <= wave_last) {
@@ -576,8 +591,7 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
     return;
   }
   if (it.part >= 0) {
-    const int64_t at = (int64_t)it.part * p.p.rows + row.place;
-    float *sums = reinterpret_cast<float *>(p.ws) + at * kD;
+    float *sums = part_of<kD>(p, it.part) + (int64_t)row.place * kD;
 #pragma unroll
     for (int i = 0; i < kDTiles; ++i) {
 #pragma unroll
@@ -587,8 +601,8 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
       }
     }
     if (g == 0) {
-      float *stats = reinterpret_cast<float *>(p.ws) + (int64_t)p.p.parts * p.p.rows * kD + at * 2;
-      *reinterpret_cast<f32x2 *>(stats) = f32x2{m_run, l_run};
+      *reinterpret_cast<f32x2 *>(part_of<kD>(p, it.part) + (int64_t)p.p.rows * kD +
+                                 (int64_t)row.place * 2) = f32x2{m_run, l_run};
     }
     return;
   }
@@ -640,12 +654,12 @@ __device__ __forceinline__ void rows16(const KernelArgs &p, const Item &it, char
   const int l16 = lane & 15;
   const int g = lane >> 4;
 
-  const Row row = row_of(p, it, l16);
-  const bool real = row.place >= 0;
-  const int lim_lo = __builtin_amdgcn_readfirstlane(wave_min(real ? row.limit : INT32_MAX));
-  const int lim_hi = __builtin_amdgcn_readfirstlane(wave_max(real ? row.limit : -1));
-  const int limit = real ? row.limit : lim_hi;
-  const int last = min(it.last - 1, block_of(it, lim_hi, kRK));
+  const Row row = row_of(p, it.kv, it.b, it.row0 + l16);
+  const bool real = row.real;
+  const Limits lim = limits_of(p, it, row);
+  const int limit = real ? row.limit : lim.hi;
+  const int lim_lo = lim.lo;
+  const int last = min(min(it.last - 1, it.end), block_of(it, lim.hi, kRK));
 
   u32x4 qf[kSteps];
 #pragma unroll
@@ -846,8 +860,8 @@ __device__ __forceinline__ void rows16(const KernelArgs &p, const Item &it, char
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int r = threadIdx.x / kQuads + i * kStep;
-    const Row to = row_of(p, it, r);
-    if (to.place < 0) {
+    const Row to = row_of(p, it.kv, it.b, it.row0 + r);
+    if (!to.real) {
       continue;
     }
     const float m = fmaxf(fmaxf(sm[0][r], sm[1][r]), fmaxf(sm[2][r], sm[3][r]));
@@ -865,11 +879,11 @@ __device__ __forceinline__ void rows16(const KernelArgs &p, const Item &it, char
       }
     }
     if (it.part >= 0) {
-      const int64_t at = (int64_t)it.part * p.p.rows + to.place;
-      float *ws = reinterpret_cast<float *>(p.ws);
-      *reinterpret_cast<f32x4 *>(ws + at * kD + c4) = acc;
+      float *part = part_of<kD>(p, it.part);
+      *reinterpret_cast<f32x4 *>(part + (int64_t)to.place * kD + c4) = acc;
       if (c4 == 0) {
-        *reinterpret_cast<f32x2 *>(ws + (int64_t)p.p.parts * p.p.rows * kD + at * 2) = f32x2{m, l};
+        *reinterpret_cast<f32x2 *>(part + (int64_t)p.p.rows * kD + (int64_t)to.place * 2) =
+            f32x2{m, l};
       }
       continue;
     }
@@ -907,6 +921,7 @@ __global__ __launch_bounds__(kThreads, 2) void flash_shared(KernelArgs p) {
     it.row0 = id / readings * (kSharedRows ? 16 : 128 / kGroups);
     it.part = p.p.parts > 1 ? split : -1;
     it.seg[1] = Segment{nullptr, nullptr, 0};
+    it.end = INT32_MAX;
     it.blocks0 = (a.shared_len + kSharedSize - 1) / kSharedSize;
     it.first = (int)((int64_t)it.blocks0 * split / p.p.shared_splits);
     it.last = (int)((int64_t)it.blocks0 * (split + 1) / p.p.shared_splits);
@@ -927,6 +942,15 @@ __global__ __launch_bounds__(kThreads, 2) void flash_shared(KernelArgs p) {
     const int64_t mine = ((int64_t)it.b * a.kv_heads + it.kv) * a.capacity * kD;
     it.seg[1] = Segment{a.k + mine, a.v + mine, own};
     it.blocks0 = (a.shared_len + kOwnSize - 1) / kOwnSize;
+    it.end = INT32_MAX;
+    if (a.causal) { /* by the last of the tile's queries, all of one head or not */
+      const int r1 = min(it.row0 + (kOwnRows ? 16 : 128 / kGroups), p.rows_seq) - 1;
+      const int i1 = it.row0 / a.seq_q == r1 / a.seq_q ? r1 % a.seq_q : a.seq_q - 1;
+      const int at = a.shared_len + own - a.seq_q + i1;
+      it.end = at < 0                ? -1
+               : at < a.shared_len ? at / kOwnSize
+                                   : it.blocks0 + (at - a.shared_len) / kOwnSize;
+    }
     /* all blocks, or those of the own keys */
     const int begin = p.p.together ? 0 : it.blocks0;
     const int blocks = it.blocks0 + (own + kOwnSize - 1) / kOwnSize - begin;
@@ -948,62 +972,97 @@ __global__ __launch_bounds__(kThreads, 2) void flash_shared(KernelArgs p) {
   }
 }
 
-/* A row's parts added up: kD / 4 threads a row, four columns each. */
-template <int kD> __global__ __launch_bounds__(kThreads) void flash_shared_merge(KernelArgs p) {
-  constexpr int kQuads = kD / 4;
-  constexpr int kBatch = 4; /* parts' loads in flight */
-  const int row = (int)(((int64_t)blockIdx.x * kThreads + threadIdx.x) / kQuads);
-  const int c4 = threadIdx.x % kQuads * 4;
-  if (row >= p.p.rows || own_keys(p.a, row / (p.a.heads * p.a.seq_q)) < 0) {
-    return;
-  }
-  const float *sums = reinterpret_cast<const float *>(p.ws) + (int64_t)row * kD + c4;
-  const float *stats = reinterpret_cast<const float *>(p.ws) + (int64_t)p.p.parts * p.p.rows * kD +
-                       (int64_t)row * 2;
+/* Four columns of a row, with the row's running maximum and weight. */
+struct Sum {
   float m = -INFINITY, l = 0.0f;
-  f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-  for (int s0 = 0; s0 < p.p.parts; s0 += kBatch) {
+  f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+
+  __device__ __forceinline__ void add(f32x2 ml, f32x4 w) {
+    const float mx = fmaxf(m, ml[0]);
+    const float m_use = mx == -INFINITY ? 0.0f : mx;
+    const float back = __builtin_amdgcn_exp2f(m - m_use);
+    const float f = __builtin_amdgcn_exp2f(ml[0] - m_use);
+    m = mx;
+    l = l * back + ml[1] * f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = v[e] * back + w[e] * f;
+    }
+  }
+  template <int kD>
+  __device__ __forceinline__ void store(const SharedAttnArgs &a, int place, int c4) const {
+    const bool seen = m > -INFINITY || l != 0.0f;
+    const float inv = seen ? 1.0f / l : 0.0f;
+    *reinterpret_cast<u32x2 *>(a.o + (int64_t)place * kD + c4) =
+        u32x2{pack2(v[0] * inv, v[1] * inv), pack2(v[2] * inv, v[3] * inv)};
+    if (a.lse && c4 == 0) {
+      a.lse[place] = seen ? (m + log2f(l)) * kLn2 : -INFINITY;
+    }
+  }
+};
+
+/* Parts first, first + step, .. of [0, parts), `get` giving one's statistics
+ * and columns; kBatch of them in flight. */
+template <int kBatch, typename F>
+__device__ __forceinline__ void add_parts(Sum &sum, int first, int step, int parts, F get) {
+  for (int s0 = first; s0 < parts; s0 += kBatch * step) {
     f32x2 ml[kBatch];
     f32x4 v[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int64_t s = min(s0 + u, p.p.parts - 1);
-      ml[u] = *reinterpret_cast<const f32x2 *>(stats + s * p.p.rows * 2);
-      v[u] = *reinterpret_cast<const f32x4 *>(sums + s * p.p.rows * kD);
-    }
-    float mx = m;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      ml[u][0] = s0 + u < p.p.parts ? ml[u][0] : -INFINITY;
-      mx = fmaxf(mx, ml[u][0]);
-    }
-    const float m_use = mx == -INFINITY ? 0.0f : mx;
-    const float back = __builtin_amdgcn_exp2f(m - m_use);
-    l *= back;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[e] *= back;
+      get(min(s0 + u * step, parts - 1), ml[u], v[u]);
     }
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      if (s0 + u < p.p.parts) {
-        const float f = __builtin_amdgcn_exp2f(ml[u][0] - m_use);
-        l += ml[u][1] * f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          acc[e] += v[u][e] * f;
-        }
+      if (s0 + u * step < parts) {
+        sum.add(ml[u], v[u]);
       }
     }
-    m = mx;
   }
-  const bool seen = m > -INFINITY || l != 0.0f;
-  const float inv = seen ? 1.0f / l : 0.0f;
-  *reinterpret_cast<u32x2 *>(p.a.o + (int64_t)row * kD + c4) =
-      u32x2{pack2(acc[0] * inv, acc[1] * inv), pack2(acc[2] * inv, acc[3] * inv)};
-  if (p.a.lse && c4 == 0) {
-    p.a.lse[row] = seen ? (m + log2f(l)) * kLn2 : -INFINITY;
+}
+
+/* kD / 4 threads a row, four columns each, and kSlices of those, which take
+ * every kSlices-th part and meet in LDS. */
+template <int kD, int kSlices>
+__global__ __launch_bounds__(kThreads) void flash_shared_merge(KernelArgs p) {
+  constexpr int kQuads = kD / 4;
+  constexpr int kOne = kThreads / kSlices;
+  const int slice = threadIdx.x / kOne, t = threadIdx.x % kOne;
+  const int row = (int)blockIdx.x * (kOne / kQuads) + t / kQuads;
+  const int c4 = t % kQuads * 4;
+  const bool real = row < p.p.rows && own_keys(p.a, row / (p.a.heads * p.a.seq_q)) >= 0;
+  Sum sum;
+  if (real) {
+    add_parts<kSlices == 1 ? 6 : 5>(sum, slice, kSlices, p.p.parts, [&](int s, f32x2 &ml, f32x4 &v) {
+      const float *part = part_of<kD>(p, s);
+      ml = *reinterpret_cast<const f32x2 *>(part + (int64_t)p.p.rows * kD + (int64_t)row * 2);
+      v = *reinterpret_cast<const f32x4 *>(part + (int64_t)row * kD + c4);
+    });
   }
+  if constexpr (kSlices > 1) {
+    __shared__ f32x4 sv[kSlices][kOne];
+    __shared__ f32x2 sml[kSlices][kOne];
+    sv[slice][t] = sum.v;
+    sml[slice][t] = f32x2{sum.m, sum.l};
+    __syncthreads();
+    if (slice != 0) {
+      return;
+    }
+#pragma unroll
+    for (int s = 1; s < kSlices; ++s) {
+      sum.add(sml[s][t], sv[s][t]);
+    }
+  }
+  if (real) {
+    sum.store<kD>(p.a, row, c4);
+  }
+}
+
+template <int kD, int kSlices> void launch_merge(const KernelArgs &k, hipStream_t stream) {
+  const int64_t threads = (int64_t)k.p.rows * (kD / 4) * kSlices;
+  hipLaunchKernelGGL((flash_shared_merge<kD, kSlices>),
+                     dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
+                     stream, k);
 }
 
 template <int kD, bool kSharedRows, int kGroups, bool kOwnRows>
@@ -1022,11 +1081,38 @@ template <int kD> void launch_all(const KernelArgs &k, hipStream_t stream) {
     k.p.tile == 64 ? launch<kD, false, 2, false>(k, stream) : launch<kD, false, 1, false>(k, stream);
   }
   if (k.p.parts > 1) {
-    const int64_t threads = (int64_t)k.p.rows * (kD / 4);
-    hipLaunchKernelGGL((flash_shared_merge<kD>),
-                       dim3((unsigned)((threads + kThreads - 1) / kThreads)), dim3(kThreads), 0,
-                       stream, k);
+    /* 65 parts of 32 rows 14 -> 6 us, 5 of 4096 rows 5.2 against 9 */
+    k.p.parts > 8 ? launch_merge<kD, 4>(k, stream) : launch_merge<kD, 1>(k, stream);
   }
+}
+
+/* Workgroups that divide the keys of each of `items` tiles: one a CU of at
+ * least 8 blocks of 64 keys, or half as many of at least 4. A workgroup costs 5
+ * us besides its blocks, and its partial results as much traffic as 130 keys:
+ * 64 sequences of 32 heads on 4 over 8192 keys (16 tiles) 30 us in 16 splits,
+ * 39 in 8 or 32; 128 sequences, 32 heads on 8, over 2048 31 in 4, 38 in 8; 16
+ * over 4096 (8 tiles) 15 in 16, 19 in 8. */
+int shared_splits(int64_t items, int64_t blocks, int cus) {
+  int64_t s = std::min(cus / items, blocks / 8);
+  if (items * s < cus / 2) {
+    s = std::min(cus / 2 / items, blocks / 4);
+  }
+  return (int)std::max<int64_t>(1, std::min<int64_t>(s, 64));
+}
+
+/* Whether tiles of one sequence's queries walk the shared keys too, each for
+ * itself: with many queries a sequence no key is read less often otherwise,
+ * and over few shared keys reading them again costs less than the merge. In
+ * us, together and apart, 16, 64 and 256 sequences of 32 heads on 8: 250 keys
+ * 8.4 and 13, 12.5 and 17, 41 and 29.5; 500 keys 10.6 and 13, 17 and 17.6, 59
+ * and 32; 1000 keys 15 and 13.7, 26 and 19; with 8 queries each, 500 keys and
+ * 4, 16 and 64 sequences 16.3 and 13.7, 16.5 and 16.5, 18 and 29. */
+bool together(int64_t items, int rows_seq, int shared_len, int cus) {
+  if (rows_seq > 64 || shared_len == 0) {
+    return true;
+  }
+  const int64_t rounds = std::max<int64_t>(1, (items + 2 * cus - 1) / (2 * cus));
+  return rounds * shared_len <= (rows_seq <= 16 || items >= cus / 2 ? 512 : 256);
 }
 
 } // namespace
@@ -1036,35 +1122,30 @@ SharedPlan flash_shared_plan(int64_t batch, int heads, int kv_heads, int seq_q, 
   SharedPlan p{};
   const int rows_seq = heads / kv_heads * seq_q;
   p.rows = (int)(batch * heads * seq_q);
-  p.parts = 1;
-  p.shared_splits = 0;
   p.own_splits = 1;
   p.own_rows = rows_seq <= 16;
   p.tile = rows_seq <= 64 ? 64 : 128;
-  p.together = true;
-  if (may_split && rows_seq <= 64 && batch > 1 && shared_len > 0) {
+  p.together = !may_split || batch == 1 || together(batch * kv_heads, rows_seq, shared_len, cus);
+  if (!p.together) {
     /* the shared keys once for rows of many sequences */
-    p.together = false;
     const int64_t rows_kv = batch * rows_seq;
     p.shared_rows = p.own_rows && rows_kv <= 16;
     p.tile = rows_kv <= 64 ? 64 : 128;
     const int tile = p.shared_rows ? 16 : p.tile;
-    const int64_t tiles = (rows_kv + tile - 1) / tile;
-    const int64_t blocks = (shared_len + kBK - 1) / kBK;
-    const int64_t items = kv_heads * tiles;
-    p.shared_splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>({2 * cus / items, blocks / 4, 64}));
+    const int64_t items = kv_heads * ((rows_kv + tile - 1) / tile);
+    p.shared_splits = shared_splits(items, (shared_len + kBK - 1) / kBK, cus);
     p.shared_groups = (int)(items * p.shared_splits);
-    if (capacity == 0) {
-      p.own_splits = 0;
-    }
+    p.own_splits = capacity > 0 ? 1 : 0;
   }
   const int own_tile = p.own_rows ? 16 : p.tile;
   p.own_tiles = (rows_seq + own_tile - 1) / own_tile;
   const int64_t items = batch * kv_heads * p.own_tiles;
   if (may_split && p.own_splits) {
+    /* up to one workgroup a CU, where it makes up for the merge (16 sequences
+     * of 32 heads on 8, 1024 own keys each: 65 us in 2 splits, 66 in 1, 68 in 4) */
     const int64_t keys = p.together ? shared_len + (int64_t)capacity : capacity;
-    p.own_splits = (int)std::max<int64_t>(1, std::min<int64_t>({2 * cus / items, keys / 256, 16}));
+    p.own_splits = (int)std::max<int64_t>(
+        1, std::min<int64_t>({cus / items, keys / (p.together && p.own_rows ? 1024 : 512), 16}));
   }
   p.own_groups = (int)(items * p.own_splits);
   p.parts = p.shared_splits + p.own_splits;
