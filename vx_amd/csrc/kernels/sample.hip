@@ -4,50 +4,55 @@
  *
  * With tokens in the order of falling logits (the lower index first among
  * equals), each setting keeps a first part of the order, so the kept tokens
- * are one: those whose logit is above a border, and the first few of those at
- * it. The draw then goes over the kept tokens by rising index and needs no
- * sort.
+ * are those above a border: a logit, and among the tokens that have it an
+ * index. The draw then goes over the kept tokens by rising index. Nothing is
+ * sorted: a border, or the drawn token, is where a running count or weight
+ * reaches some amount, found by histograms over ever smaller ranges of an
+ * order-preserving 32-bit key (`descend`).
  *
  * Weights 2^((l - top) c), with c = log2(e) / T and top the largest logit, are
  * taken in 64 bits and kept as 64-bit integers of unit 2^-shift, so many that
- * a row's sum stays within 2^62. Integer sums do not
- * depend on their order: LDS atomics and any division of the row give the
- * same bits.
+ * a row's sum stays within 2^62. Integer sums do not depend on their order:
+ * LDS atomics and any division of the row give the same bits.
  *
- * sample_rows: a workgroup a row. A border is found digit by digit (11, 11 and
- * 10 bits) of the logits' order-preserving 32-bit keys, each digit by a
- * histogram of counts and weights over the row.
+ * A first histogram over (top - l) c finds the bin of the border of top-k (by
+ * count, no weight is taken) or of top-p (by weight). The tokens down to that
+ * bin, mostly a few dozen, then go into LDS and everything else happens there;
+ * where they are many, `descend` and the draw go over the row again.
+ *
+ * sample_rows: a workgroup a row, which it keeps in LDS up to 128 KiB of it. sample_tops and sample_parts: several workgroups a row find its
+ * top, then its histogram or weight, in a workspace; the last of a row to
+ * finish does the rest.
  */
 #include "../vx_batch_kernels.h"
 #include "../vx_hip_common.h"
+#include "vx_lds_dma.hip.h"
+#include "vx_wave_ops.hip.h"
 
+#include <algorithm>
 #include <cmath>
 
 namespace vxk {
 namespace {
 
 typedef unsigned long long u64;
+typedef uint32_t u32;
 
 constexpr int kThreads = 1024;
 constexpr int kWaves = kThreads / 64;
-constexpr int kBins = 2048;
+constexpr int kBins = 1024;      /* one a thread */
+constexpr int kChunk = 4 * kThreads; /* logits of a vector load of every thread */
+constexpr int kList = kThreads;  /* tokens in LDS, one a thread */
+constexpr int kFew = 128;        /* of which one wave handles */
+constexpr float kPerOctave = 16.0f; /* bins per factor of two of the weight: 64 of them in all */
 
-/* A row's logit in f32; -0 as +0. */
-template <bool kF32> __device__ __forceinline__ float logit(const void *row, int i) {
-  if constexpr (kF32) {
-    return static_cast<const float *>(row)[i] + 0.0f;
-  } else {
-    return bf16_to_f32(static_cast<const uint16_t *>(row)[i]) + 0.0f;
-  }
-}
-
-/* Rises with l; 0 for NaN and -inf, which are never drawn. */
-__device__ __forceinline__ uint32_t key_of(float l) {
-  const uint32_t b = __float_as_uint(l);
-  const uint32_t k = b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+/* Rises with l; 0 for -inf (and what counts as it), which is never drawn. */
+__device__ __forceinline__ u32 key_of(float l) {
+  const u32 b = __float_as_uint(l);
+  const u32 k = b ^ ((u32)((int32_t)b >> 31) | 0x80000000u);
   return l > -INFINITY ? k : 0u;
 }
-__device__ __forceinline__ float logit_of(uint32_t key) {
+__device__ __forceinline__ float logit_of(u32 key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
@@ -73,53 +78,13 @@ __device__ __forceinline__ double exp2_neg(double d) {
   return ldexp(y, (int)k);
 }
 
-/* How a row's logits become weights. */
-struct Scale {
-  double c, top; /* 2^((l - top) c) */
-  double unit; /* 2^shift */
-  bool inf;    /* a logit is +inf: those alone */
-};
-
-__device__ __forceinline__ double ratio(const Scale &s, float l) {
-  if (s.inf) {
-    return l == INFINITY ? 1.0 : 0.0;
-  }
-  return l > -INFINITY ? exp2_neg(((double)l - s.top) * s.c) : 0.0;
-}
-__device__ __forceinline__ u64 weight(const Scale &s, float l) {
-  return (u64)rint(ratio(s, l) * s.unit);
-}
-
-__device__ __forceinline__ u64 wave_max64(u64 v) {
-  for (int o = 32; o; o >>= 1) {
-    const u64 w = __shfl_xor(v, o);
-    v = w > v ? w : v;
-  }
-  return v;
-}
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-  for (int o = 32; o; o >>= 1) {
-    v += __shfl_xor(v, o);
-  }
-  return v;
-}
-/* Inclusive, over the wave's lanes up to this one. */
-__device__ __forceinline__ u64 wave_scan64(u64 v) {
-  const int lane = threadIdx.x & 63;
-  for (int o = 1; o < 64; o <<= 1) {
-    const u64 w = __shfl_up(v, o);
-    v += lane >= o ? w : 0;
-  }
-  return v;
-}
-
 /* floor(x total) and, with kUp, ceil(x total) of x in (0, 1), exactly: x is 24
  * bits times a power of two. A border that falls between two tokens (equal
  * logits, a half) falls on the side that the definition says. */
 template <bool kUp> __device__ __forceinline__ u64 part_of(float x, u64 total) {
-  const uint32_t b = __float_as_uint(x);
+  const u32 b = __float_as_uint(x);
   const int e = (int)(b >> 23);
-  const uint32_t m = (b & 0x7fffffu) | (e ? 0x800000u : 0u);
+  const u32 m = (b & 0x7fffffu) | (e ? 0x800000u : 0u);
   const int down = e ? 150 - e : 149; /* 24 .. 149 */
   const unsigned __int128 p = (unsigned __int128)m * total;
   if (down >= 128) {
@@ -129,259 +94,734 @@ template <bool kUp> __device__ __forceinline__ u64 part_of(float x, u64 total) {
   return q + (kUp && ((unsigned __int128)q << down) != p ? 1 : 0);
 }
 
-/* The border of a setting: tokens of a key above `key` stay, and the first
- * `ties` of those that have it. */
-struct Border {
-  uint32_t key;
-  u64 ties;
-  u64 mass; /* of all that stay */
+/* A row's settings, as the kernels use them. */
+struct Settings {
+  int top_k; /* 0: off */
+  float top_p, min_p;
+  bool first; /* only the first token of the order stays */
+  double c;
+  float per; /* bins per unit of logit */
 };
-
-struct Shared {
-  u64 mass[kBins];
-  uint32_t count[kBins];
-  u64 wave[kWaves], wave2[kWaves];
-  int bin;
-  u64 above_mass, above_count, bin_mass, bin_count;
-};
-
-template <bool kF32, typename F>
-__device__ __forceinline__ void each(const void *row, int vocab, F f) {
-  for (int i = threadIdx.x; i < vocab; i += kThreads) {
-    f(i, logit<kF32>(row, i));
-  }
-}
-
-/* The border at the `want`-th token (kMass false) or the token whose weights
- * from the first on reach `want`. Every thread calls it and gets the same. */
-template <bool kF32, bool kMass>
-__device__ Border find_border(Shared &sh, const void *row, int vocab, const Scale &s, u64 want) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  uint32_t prefix = 0, mask = 0;
-  u64 above_mass = 0, above_count = 0, mass = 0, count = 0;
-  constexpr int kShift[3] = {21, 10, 0};
-  for (int level = 0; level < 3; ++level) {
-    const int shift = kShift[level];
-    const uint32_t digits = level == 2 ? 1023 : 2047;
-    for (int b = t; b < kBins; b += kThreads) {
-      sh.mass[b] = 0;
-      sh.count[b] = 0;
-    }
-    __syncthreads();
-    each<kF32>(row, vocab, [&](int, float l) {
-      const uint32_t k = key_of(l);
-      if (k && (k & mask) == prefix) {
-        const int b = (int)(k >> shift & digits);
-        atomicAdd(&sh.mass[b], weight(s, l));
-        atomicAdd(&sh.count[b], 1u);
-      }
-    });
-    __syncthreads();
-    /* From the highest digit down, two a thread. */
-    const int hi = kBins - 1 - 2 * t;
-    const u64 m0 = sh.mass[hi], m1 = sh.mass[hi - 1];
-    const u64 c0 = sh.count[hi], c1 = sh.count[hi - 1];
-    const u64 ms = wave_scan64(m0 + m1), cs = wave_scan64(c0 + c1);
-    if (lane == 63) {
-      sh.wave[wave] = ms;
-      sh.wave2[wave] = cs;
-    }
-    __syncthreads();
-    u64 mb = above_mass + ms - m0 - m1, cb = above_count + cs - c0 - c1;
-    for (int w = 0; w < wave; ++w) {
-      mb += sh.wave[w];
-      cb += sh.wave2[w];
-    }
-    const u64 before = kMass ? mb : cb, own0 = kMass ? m0 : c0, own1 = kMass ? m1 : c1;
-    if (before < want && want <= before + own0) {
-      sh.bin = hi;
-      sh.above_mass = mb;
-      sh.above_count = cb;
-      sh.bin_mass = m0;
-      sh.bin_count = c0;
-    } else if (before + own0 < want && want <= before + own0 + own1) {
-      sh.bin = hi - 1;
-      sh.above_mass = mb + m0;
-      sh.above_count = cb + c0;
-      sh.bin_mass = m1;
-      sh.bin_count = c1;
-    }
-    __syncthreads();
-    prefix |= (uint32_t)sh.bin << shift;
-    mask |= digits << shift;
-    above_mass = sh.above_mass;
-    above_count = sh.above_count;
-    mass = sh.bin_mass;
-    count = sh.bin_count;
-    __syncthreads();
-  }
-  const u64 each_mass = mass / count; /* equal keys, equal weights */
-  u64 ties = kMass ? (want - above_mass + each_mass - 1) / each_mass : want - above_count;
-  ties = ties < count ? ties : count;
-  return Border{prefix, ties, above_mass + ties * each_mass};
-}
-
-template <bool kF32> __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
-  __shared__ Shared sh;
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int r = blockIdx.x;
-  const void *row = kF32 ? (const void *)(static_cast<const float *>(a.logits) + r * a.stride)
-                         : (const void *)(static_cast<const uint16_t *>(a.logits) + r * a.stride);
+__device__ __forceinline__ Settings settings_of(const SampleArgs &a, int r) {
   const float heat = a.temperature ? a.temperature[r] : 1.0f;
   const int top_k = a.top_k ? a.top_k[r] : 0;
   const float top_p = a.top_p ? a.top_p[r] : 1.0f;
   const float min_p = a.min_p ? a.min_p[r] : 0.0f;
-
-  /* The first token: the largest key, its lowest index. */
-  u64 best = 0;
-  each<kF32>(row, a.vocab, [&](int i, float l) {
-    const uint32_t k = key_of(l);
-    const u64 v = k ? (u64)k << 32 | (uint32_t)~i : 0;
-    best = v > best ? v : best;
-  });
-  best = wave_max64(best);
-  if (lane == 0) {
-    sh.wave[wave] = best;
-  }
-  __syncthreads();
-  for (int w = 0; w < kWaves; ++w) {
-    best = sh.wave[w] > best ? sh.wave[w] : best;
-  }
-  __syncthreads();
-  const bool first_alone = !(heat > 0.0f) || top_k == 1 || top_p <= 0.0f;
-  if (!best || first_alone) {
-    if (t == 0) {
-      a.tokens[r] = best ? (int)~(uint32_t)best : -1;
-      if (a.logprob) {
-        a.logprob[r] = best ? 0.0f : -INFINITY;
-      }
-    }
-    return;
-  }
-
-  const float top = logit_of((uint32_t)(best >> 32));
-  Scale s;
-  s.inf = top == INFINITY;
+  Settings s;
+  s.first = !(heat > 0.0f) || top_k == 1 || top_p <= 0.0f;
+  s.top_k = top_k > 0 && top_k < a.vocab ? top_k : 0;
+  s.top_p = top_p < 1.0f ? top_p : 1.0f;
+  s.min_p = min_p > 0.0f ? fminf(min_p, 1.0f) : 0.0f;
   s.c = 1.4426950408889634074 / (double)heat;
-  s.top = (double)top;
-  const int shift = 62 - (a.vocab > 1 ? 32 - __clz(a.vocab - 1) : 0);
-  s.unit = ldexp(1.0, shift);
+  s.per = (float)fmin(s.c * (double)kPerOctave, 1e30);
+  return s;
+}
 
-  Border border{0, ~0ull, 0};
-  if (top_k > 0 && top_k < a.vocab) {
-    /* as many as there are above -inf: all of them */
-    u64 some = 0;
-    each<kF32>(row, a.vocab, [&](int, float l) { some += l > -INFINITY; });
-    some = wave_sum64(some);
-    if (lane == 0) {
-      sh.wave[wave] = some;
-    }
-    __syncthreads();
-    some = 0;
-    for (int w = 0; w < kWaves; ++w) {
-      some += sh.wave[w];
-    }
-    __syncthreads();
-    if ((u64)top_k < some) {
-      border = find_border<kF32, false>(sh, row, a.vocab, s, (u64)top_k);
-    }
-  }
-  if (top_p < 1.0f) {
-    u64 mass = border.mass;
-    if (!border.key) {
-      each<kF32>(row, a.vocab, [&](int, float l) { mass += weight(s, l); });
-      mass = wave_sum64(mass);
-      if (lane == 0) {
-        sh.wave[wave] = mass;
-      }
-      __syncthreads();
-      mass = 0;
-      for (int w = 0; w < kWaves; ++w) {
-        mass += sh.wave[w];
-      }
-      __syncthreads();
-    }
-    const u64 want = part_of<true>(top_p, mass);
-    border = find_border<kF32, true>(sh, row, a.vocab, s, want);
-  }
+/* How a row's logits become weights. Where a logit is +inf, those count as 0
+ * and the others as -inf. */
+struct Scale {
+  double c, top, unit;
+  float ftop, per;
+  bool inf;
 
-  /* A wave's part of the row: its kept weight above the border, and its ties. */
-  const double least = min_p > 0.0f ? fmin((double)min_p, 1.0) : 0.0;
-  auto stays = [&](float l, uint32_t k) { return k >= border.key && ratio(s, l) >= least; };
-  const int per = ((a.vocab + kWaves - 1) / kWaves + 63) / 64 * 64;
-  const int i0 = min(a.vocab, wave * per), i1 = min(a.vocab, i0 + per);
-  u64 mass = 0, ties = 0;
-  for (int i = i0 + lane; i < i1; i += 64) {
-    const float l = logit<kF32>(row, i);
-    const uint32_t k = key_of(l);
-    if (k && stays(l, k)) {
-      if (k == border.key) {
-        ++ties;
-      } else {
-        mass += weight(s, l);
-      }
-    }
+  __device__ __forceinline__ float logit(float l) const {
+    return !inf ? l : l == INFINITY ? 0.0f : -INFINITY;
   }
-  mass = wave_sum64(mass);
-  ties = wave_sum64(ties);
-  if (lane == 0) {
-    sh.wave[wave] = mass;
-    sh.wave2[wave] = ties;
+  /* of what logit() gives */
+  __device__ __forceinline__ double ratio(float l) const {
+    return exp2_neg(((double)l - top) * c); /* 0 for -inf */
+  }
+  __device__ __forceinline__ u64 weight(float l) const { return (u64)rint(ratio(l) * unit); }
+  /* Falls with l; the last bin's weights are 0. */
+  __device__ __forceinline__ int bin(float l) const {
+    return (int)fminf(fminf(ftop - l, 3.4028234664e38f) * per, (float)(kBins - 1));
+  }
+};
+__device__ __forceinline__ Scale scale_of(const SampleArgs &a, const Settings &s, float top) {
+  Scale x;
+  x.inf = top == INFINITY;
+  x.ftop = x.inf ? 0.0f : top;
+  x.top = (double)x.ftop;
+  x.c = s.c;
+  x.per = s.per;
+  x.unit = ldexp(1.0, 62 - (a.vocab > 1 ? 32 - __clz(a.vocab - 1) : 0));
+  return x;
+}
+
+__device__ __forceinline__ u64 wave_sum64(u64 v) {
+  for (int o = 32; o; o >>= 1) {
+    v += __shfl_xor(v, o);
+  }
+  return v;
+}
+/* Inclusive, over the wave's lanes up to this one. */
+template <typename T> __device__ __forceinline__ T wave_scan(T v) {
+  const int lane = threadIdx.x & 63;
+  for (int o = 1; o < 64; o <<= 1) {
+    const T w = __shfl_up(v, o);
+    v += lane >= o ? w : 0;
+  }
+  return v;
+}
+
+struct Found {
+  u64 above_mass, mass;
+  u32 above_count, count;
+  int bin;
+};
+
+struct Shared {
+  u64 mass[kBins];
+  u64 list_w[kList];
+  u64 list_k[kList]; /* key, then the index's complement */
+  u32 count[kBins];
+  u64 wave_m[kWaves];
+  u32 wave_c[kWaves];
+  u32 n;
+  Found found;
+};
+
+__device__ __forceinline__ u64 block_sum(Shared &sh, u64 v) {
+  v = wave_sum64(v);
+  if ((threadIdx.x & 63) == 0) {
+    sh.wave_m[threadIdx.x >> 6] = v;
   }
   __syncthreads();
-  const u64 tie_weight = border.key ? weight(s, logit_of(border.key)) : 0;
-  u64 total = 0, before = 0, left = border.ties, my_left = 0;
+  u64 sum = 0;
+#pragma unroll
   for (int w = 0; w < kWaves; ++w) {
-    if (w == wave) {
-      before = total;
-      my_left = left;
-    }
-    const u64 n = sh.wave2[w] < left ? sh.wave2[w] : left;
-    total += sh.wave[w] + n * tie_weight;
-    left -= n;
+    sum += sh.wave_m[w];
   }
-  float u = a.u[r];
-  u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
-  u64 target = part_of<false>(u, total);
-  const u64 mine = mass + (ties < my_left ? ties : my_left) * tie_weight;
-  if (target < before || target >= before + mine) {
-    return;
+  __syncthreads();
+  return sum;
+}
+__device__ __forceinline__ float block_max(Shared &sh, float v) {
+  v = wave_max(v);
+  if ((threadIdx.x & 63) == 0) {
+    sh.wave_c[threadIdx.x >> 6] = __float_as_uint(v);
   }
-  target -= before;
-  for (int i = i0; i < i1; i += 64) {
-    const bool in = i + lane < i1;
-    const float l = in ? logit<kF32>(row, i + lane) : -INFINITY;
-    const uint32_t k = key_of(l);
-    const bool kept = k && stays(l, k);
-    const bool tie = kept && k == border.key;
-    const u64 tied = __ballot(tie);
-    const bool over = tie && (u64)__popcll(tied & ((1ull << lane) - 1)) >= my_left;
-    const u64 w = kept && !over ? weight(s, l) : 0;
-    const u64 sum = wave_scan64(w);
-    const u64 hit = __ballot(sum > target);
-    if (hit) {
-      if (lane == __ffsll((long long)hit) - 1) {
-        a.tokens[r] = i + lane;
-        if (a.logprob) {
-          a.logprob[r] = (float)log((double)w / (double)total);
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    v = fmaxf(v, __uint_as_float(sh.wave_c[w]));
+  }
+  __syncthreads();
+  return v;
+}
+
+/* Which bin a running count or weight over the threads' bins, from thread 0 on,
+ * starts at from `above_*` and reaches `want` in; there is one. */
+template <bool kMass>
+__device__ Found find_bin(Shared &sh, u64 mass, u32 count, u64 above_mass, u32 above_count,
+                          u64 want) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const u64 ms = wave_scan(mass);
+  const u32 cs = wave_scan(count);
+  if (lane == 63) {
+    sh.wave_m[wave] = ms;
+    sh.wave_c[wave] = cs;
+  }
+  __syncthreads();
+  u64 mb = above_mass + ms - mass;
+  u32 cb = above_count + cs - count;
+  for (int w = 0; w < wave; ++w) {
+    mb += sh.wave_m[w];
+    cb += sh.wave_c[w];
+  }
+  const u64 before = kMass ? mb : cb, own = kMass ? mass : count;
+  if (before < want && want <= before + own) {
+    sh.found = Found{mb, mass, cb, count, (int)threadIdx.x};
+  }
+  __syncthreads();
+  const Found f = sh.found;
+  __syncthreads();
+  return f;
+}
+
+/* Over the items that `each` gives to its callback (a key, and what makes its
+ * weight), in the order of falling keys: the key at which the running count
+ * (kMass: weight), `above` items above `hi` included, reaches `want`; with the
+ * sums above it and at it. Keys outside [lo, hi] are passed over. */
+struct Point {
+  u32 key;
+  Found f;
+};
+template <bool kMass, typename Each>
+__device__ Point descend(Shared &sh, Each each, u32 lo, u32 hi, u64 above_mass, u32 above_count,
+                         u64 want) {
+  const int t = threadIdx.x;
+  for (;;) {
+    const u32 width = hi - lo;
+    const int shift = max(0, 32 - (width ? __clz((int)width) : 32) - 10);
+    sh.mass[t] = 0;
+    sh.count[t] = 0;
+    __syncthreads();
+    each([&](u32 key, auto weight) {
+      if (key >= lo && key <= hi) {
+        const u32 b = (hi - key) >> shift;
+        if constexpr (kMass) {
+          atomicAdd(&sh.mass[b], weight());
         }
+        atomicAdd(&sh.count[b], 1u);
+      }
+    });
+    __syncthreads();
+    const Found f = find_bin<kMass>(sh, sh.mass[t], sh.count[t], above_mass, above_count, want);
+    hi -= (u32)f.bin << shift;
+    if (shift == 0) {
+      return Point{hi, f};
+    }
+    const u32 span = (1u << shift) - 1;
+    lo = hi - lo > span ? hi - span : lo;
+    above_mass = f.above_mass;
+    above_count = f.above_count;
+  }
+}
+
+/* Tokens that stay: keys above `key`, and those that have it up to index
+ * `last`. */
+struct Border {
+  u32 key, last;
+  __device__ __forceinline__ bool keeps(u32 k, u32 i) const {
+    return k > key || (k == key && i <= last);
+  }
+};
+
+/* The border at `point`, whose first `ties` tokens stay. */
+template <typename Each>
+__device__ Border border_at(Shared &sh, Each each, const Point &point, u64 ties, int vocab) {
+  if (ties >= point.f.count) {
+    return Border{point.key, 0xffffffffu};
+  }
+  const Point p = descend<false>(
+      sh,
+      [&](auto take) {
+        each([&](u32 key, u32 i, auto) {
+          if (key == point.key) {
+            take(~i, [] { return u64(0); });
+          }
+        });
+      },
+      ~(u32)(vocab - 1), 0xffffffffu, 0, 0, ties);
+  return Border{point.key, ~p.key};
+}
+
+/* How many of the tokens at a point stay where a running weight stops at
+ * `want`: those before which it is less. */
+__device__ __forceinline__ u64 ties_of(const Found &f, u64 want) {
+  const u64 each = f.mass / f.count; /* equal keys, equal weights */
+  return (want - f.above_mass + each - 1) / each;
+}
+
+__device__ __forceinline__ u64 target_of(const SampleArgs &a, int r, u64 total) {
+  const float u = a.u[r];
+  return part_of<false>(u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f, total);
+}
+
+__device__ __forceinline__ void put(const SampleArgs &a, int r, int token, u64 w, u64 total) {
+  a.tokens[r] = token;
+  if (a.logprob) {
+    a.logprob[r] = (float)log((double)w / (double)total);
+  }
+}
+
+/* Everything that is left to do for at most kFew tokens in the list, by one
+ * wave, two tokens a lane. `mass`: the weight that top_p is a share of, where
+ * no top_k is on. */
+__device__ void finish_few(const SampleArgs &a, Shared &sh, int r, const Settings &s,
+                           const Scale &x, int n, u64 mass) {
+  const int lane = threadIdx.x;
+  u64 k[2], w[2], before[2] = {0, 0};
+  u32 rank[2] = {0, 0};
+  bool in[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    in[e] = lane + 64 * e < n;
+    k[e] = in[e] ? sh.list_k[lane + 64 * e] : 0;
+    w[e] = in[e] ? sh.list_w[lane + 64 * e] : 0;
+  }
+  for (int j = 0; j < n; ++j) {
+    const u64 kj = sh.list_k[j], wj = sh.list_w[j];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bool over = kj > k[e];
+      rank[e] += over ? 1u : 0u;
+      before[e] += over ? wj : 0;
+    }
+  }
+  if (s.top_k) {
+    mass = 0;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      in[e] = in[e] && rank[e] < (u32)s.top_k;
+      mass += in[e] ? w[e] : 0;
+    }
+    mass = wave_sum64(mass);
+  }
+  if (s.top_p < 1.0f) {
+    const u64 want = part_of<true>(s.top_p, mass);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      in[e] = in[e] && before[e] < want;
+    }
+  }
+  u64 total = 0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (s.min_p > 0.0f) {
+      in[e] = in[e] && x.ratio(logit_of((u32)(k[e] >> 32))) >= (double)s.min_p;
+    }
+    w[e] = in[e] ? w[e] : 0;
+    total += w[e];
+    if (lane + 64 * e < n) {
+      sh.list_w[lane + 64 * e] = w[e];
+    }
+  }
+  total = wave_sum64(total);
+  const u64 target = target_of(a, r, total);
+  u64 upto[2] = {0, 0}; /* over the tokens of lower indexes */
+  for (int j = 0; j < n; ++j) {
+    const u32 ij = ~(u32)sh.list_k[j];
+    const u64 wj = sh.list_w[j];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      upto[e] += ij < ~(u32)k[e] ? wj : 0;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (in[e] && upto[e] <= target && target < upto[e] + w[e]) {
+      put(a, r, (int)~(u32)k[e], w[e], total);
+    }
+  }
+}
+
+/* The same for up to kList tokens, one a thread, of bins up to `bin`. */
+__device__ void finish_list(const SampleArgs &a, Shared &sh, int r, const Settings &s,
+                            const Scale &x, int n, u64 mass, int bin) {
+  const int t = threadIdx.x;
+  const bool mine = t < n;
+  const u64 kw = mine ? sh.list_k[t] : 0;
+  const u64 w = mine ? sh.list_w[t] : 0;
+  const u32 key = (u32)(kw >> 32), i = ~(u32)kw;
+  bool in = mine;
+  const u32 hi = key_of(x.ftop);
+  const float least = x.per > 0.0f ? x.ftop - (float)(bin + 2) / x.per : -INFINITY;
+  const u32 lo = max(key_of(least), 1u); /* a bin below the last one's end */
+  auto by_key = [&](auto take) {
+    if (in) {
+      take(key, [&] { return w; });
+    }
+  };
+  auto both = [&](auto take) {
+    if (in) {
+      take(key, i, [&] { return w; });
+    }
+  };
+  if (s.top_k) {
+    const Point p = descend<false>(sh, by_key, lo, hi, 0, 0, (u64)s.top_k);
+    const Border b = border_at(sh, both, p, (u64)s.top_k - p.f.above_count, a.vocab);
+    in = mine && b.keeps(key, i);
+    mass = s.top_p < 1.0f ? block_sum(sh, in ? w : 0) : 0;
+  }
+  if (s.top_p < 1.0f) {
+    const u64 want = part_of<true>(s.top_p, mass);
+    const Point p = descend<true>(sh, by_key, lo, hi, 0, 0, want);
+    const Border b = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
+    in = in && b.keeps(key, i);
+  }
+  if (s.min_p > 0.0f) {
+    in = in && x.ratio(logit_of(key)) >= (double)s.min_p;
+  }
+  const u64 total = block_sum(sh, in ? w : 0);
+  const u64 target = target_of(a, r, total);
+  const Point p = descend<true>(
+      sh,
+      [&](auto take) {
+        if (in) {
+          take(~i, [&] { return w; });
+        }
+      },
+      ~(u32)(a.vocab - 1), 0xffffffffu, 0, 0, target + 1);
+  if (in && i == ~p.key) {
+    put(a, r, (int)i, w, total);
+  }
+}
+
+/* Four logits from index i on (NaN as -inf, -0 as +0), -inf from `end` on. */
+template <bool kF32> struct Four;
+template <> struct Four<true> {
+  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
+  typedef float whole __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ float value(float v) { return v; }
+};
+template <> struct Four<false> {
+  typedef unsigned short type __attribute__((ext_vector_type(4), aligned(2)));
+  typedef unsigned short whole __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ float value(unsigned short v) { return bf16_to_f32(v); }
+};
+
+/* A row, in memory or (kLds bytes, room for all of it) in LDS. */
+template <bool kF32, int kLds> struct Row {
+  typedef typename Four<kF32>::type V;
+  typedef typename Four<kF32>::whole VA;
+  static constexpr int kSize = kF32 ? 4 : 2;
+  const char *p;
+  int vocab;
+  u32 lds; /* where LDS holds it */
+
+  __device__ __forceinline__ Row(const SampleArgs &a, int r, const char *buffer)
+      : p(static_cast<const char *>(a.logits) + (int64_t)r * a.stride * kSize), vocab(a.vocab),
+        lds(kLds ? (u32)(uintptr_t)(const VX_LDS char *)buffer : 0u) {}
+
+  static __device__ __forceinline__ float clean(float l) {
+    return l > -INFINITY ? l + 0.0f : -INFINITY;
+  }
+  __device__ __forceinline__ void from_memory(int64_t i, int64_t end, float (&l)[4]) const {
+    if (i + 3 < end) {
+      const V v = *reinterpret_cast<const V *>(p + i * kSize);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        l[e] = clean(Four<kF32>::value(v[e]));
       }
       return;
     }
-    target -= __shfl(sum, 63);
-    const u64 n = (u64)__popcll(tied);
-    my_left -= n < my_left ? n : my_left;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      l[e] = -INFINITY;
+      if (i + e < end) {
+        if constexpr (kF32) {
+          l[e] = clean(reinterpret_cast<const float *>(p)[i + e]);
+        } else {
+          l[e] = clean(bf16_to_f32(reinterpret_cast<const uint16_t *>(p)[i + e]));
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void load4(int64_t i, int64_t end, float (&l)[4]) const {
+    if constexpr (kLds > 0) {
+      const VA v = *(const VX_LDS VA *)(uintptr_t)(lds + (u32)i * kSize);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        l[e] = i + e < end ? clean(Four<kF32>::value(v[e])) : -INFINITY;
+      }
+    } else {
+      from_memory(i, end, l);
+    }
+  }
+  /* The row's first reading: its largest logit, and into LDS. */
+  __device__ __forceinline__ float take() const {
+    float top = -INFINITY;
+#pragma unroll 4
+    for (int64_t i = 4 * threadIdx.x; i < vocab; i += kChunk) {
+      float l[4];
+      from_memory(i, vocab, l);
+      VA v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        top = fmaxf(top, l[e]);
+        if constexpr (kF32) {
+          v[e] = l[e];
+        } else {
+          v[e] = (unsigned short)(__float_as_uint(l[e]) >> 16); /* as it was, but for NaN */
+        }
+      }
+      if constexpr (kLds > 0) {
+        *(VX_LDS VA *)(uintptr_t)(lds + (u32)i * kSize) = v;
+      }
+    }
+    return top;
+  }
+  /* f(index, logit), in no order. */
+  template <typename F> __device__ __forceinline__ void each(F f) const {
+#pragma unroll 1
+    for (int64_t i = 4 * threadIdx.x; i < vocab; i += kChunk) {
+      float v[4];
+      load4(i, vocab, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f((u32)i + e, v[e]);
+      }
+    }
+  }
+};
+
+/* The draw over a row, `weight` giving a token's (0 if it does not stay). The
+ * row, then the part of it that the sum falls in, is cut into a part for each
+ * wave until it is a chunk. */
+template <typename R, typename W>
+__device__ void draw(const SampleArgs &a, Shared &sh, int r, const R &row, W weight) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  int64_t begin = 0, end = row.vocab;
+  u64 total = 0, target = 0;
+  while (end - begin > kChunk) {
+    const int64_t per = ((end - begin + kWaves - 1) / kWaves + 3) / 4 * 4;
+    const int64_t i0 = begin + wave * per, i1 = i0 + per < end ? i0 + per : end;
+    u64 sum = 0;
+#pragma unroll 1
+    for (int64_t i = i0 + 4 * lane; i < i1; i += 256) {
+      float v[4];
+      row.load4(i, i1, v);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        sum += weight((u32)(i + e), v[e]);
+      }
+    }
+    sum = wave_sum64(sum);
+    if (lane == 0) {
+      sh.wave_m[wave] = sum;
+    }
+    __syncthreads();
+    if (total == 0) {
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        total += sh.wave_m[w];
+      }
+      target = target_of(a, r, total);
+    }
+    int at = 0;
+    for (; at + 1 < kWaves && target >= sh.wave_m[at]; ++at) {
+      target -= sh.wave_m[at];
+    }
+    __syncthreads();
+    begin += at * per;
+    end = begin + per < end ? begin + per : end;
+  }
+  float v[4];
+  u64 w[4], sum = 0;
+  const int64_t i = begin + 4 * t;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    v[e] = -INFINITY;
+  }
+  if (i < end) {
+    row.load4(i, end, v);
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    w[e] = weight((u32)(i + e), v[e]);
+    sum += w[e];
+  }
+  if (total == 0) {
+    total = block_sum(sh, sum);
+    target = target_of(a, r, total);
+  }
+  const Found f = find_bin<true>(sh, sum, 0, 0, 0, target + 1);
+  if (f.bin == t) {
+    target -= f.above_mass;
+    for (int e = 0; e < 4; ++e) {
+      if (target < w[e]) {
+        put(a, r, (int)(i + e), w[e], total);
+        return;
+      }
+      target -= w[e];
+    }
+  }
+}
+
+/* What is left to do once the row's histogram is in the threads' registers
+ * (`mass` only where no top_k is on; all of the row's bins). */
+template <typename R>
+__device__ void finish_bins(const SampleArgs &a, Shared &sh, int r, const R &row, Settings s,
+                            const Scale &x, u64 mass, u32 count) {
+  const int t = threadIdx.x;
+  u64 sum = 0;
+  Found f;
+  if (s.top_k) {
+    /* more than there are above -inf, or into the weights of 0: all of them */
+    const u64 all = block_sum(sh, t == kBins - 1 ? 0 : count);
+    if ((u64)s.top_k > all) {
+      s.top_k = 0;
+      if (s.top_p < 1.0f) {
+        sh.mass[t] = 0;
+        __syncthreads();
+        row.each([&](u32, float l) {
+          l = x.logit(l);
+          if (l > -INFINITY) {
+            atomicAdd(&sh.mass[x.bin(l)], x.weight(l));
+          }
+        });
+        __syncthreads();
+        mass = sh.mass[t];
+      }
+    } else {
+      f = find_bin<false>(sh, 0, count, 0, 0, (u64)s.top_k);
+    }
+  }
+  if (!s.top_k && s.top_p < 1.0f) {
+    sum = block_sum(sh, mass);
+    f = find_bin<true>(sh, mass, count, 0, 0, part_of<true>(s.top_p, sum));
+  }
+  const bool bordered = s.top_k || s.top_p < 1.0f;
+  if (bordered && f.above_count + f.count <= (u32)kList) {
+    const int n = (int)(f.above_count + f.count);
+    if (t == 0) {
+      sh.n = 0;
+    }
+    __syncthreads();
+    row.each([&](u32 i, float l) {
+      l = x.logit(l);
+      if (l > -INFINITY && x.bin(l) <= f.bin) {
+        const u32 at = atomicAdd(&sh.n, 1u);
+        sh.list_k[at] = (u64)key_of(l) << 32 | (u32)~i;
+      }
+    });
+    __syncthreads();
+    if (n <= kFew) {
+      if (t < 64) {
+        for (int j = t; j < n; j += 64) {
+          sh.list_w[j] = x.weight(logit_of((u32)(sh.list_k[j] >> 32)));
+        }
+        finish_few(a, sh, r, s, x, n, sum);
+      }
+      return;
+    }
+    if (t < n) {
+      sh.list_w[t] = x.weight(logit_of((u32)(sh.list_k[t] >> 32)));
+    }
+    finish_list(a, sh, r, s, x, n, sum, f.bin);
+    return;
+  }
+  Border border{0, 0xffffffffu};
+  if (bordered) {
+    auto by_key = [&](auto take) {
+      row.each([&](u32 i, float l) {
+        l = x.logit(l);
+        const u32 k = key_of(l);
+        if (k && border.keeps(k, i)) {
+          take(k, [&] { return x.weight(l); });
+        }
+      });
+    };
+    auto both = [&](auto take) {
+      row.each([&](u32 i, float l) {
+        l = x.logit(l);
+        const u32 k = key_of(l);
+        if (k && border.keeps(k, i)) {
+          take(k, i, [&] { return x.weight(l); });
+        }
+      });
+    };
+    /* from the top to a bin below the border's */
+    const float per = x.per;
+    const u32 lo = max(per > 0.0f ? key_of(x.ftop - (float)(f.bin + 2) / per) : 0u, 1u);
+    const u32 hi = key_of(x.ftop);
+    if (s.top_k) {
+      const Point p = descend<false>(sh, by_key, lo, hi, 0, 0, (u64)s.top_k);
+      border = border_at(sh, both, p, (u64)s.top_k - p.f.above_count, a.vocab);
+      if (s.top_p < 1.0f) {
+        by_key([&](u32, auto weight) { sum += weight(); });
+        sum = block_sum(sh, sum);
+      }
+    }
+    if (s.top_p < 1.0f) {
+      const u64 want = part_of<true>(s.top_p, sum);
+      const Point p = descend<true>(sh, by_key, lo, hi, 0, 0, want);
+      border = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
+    }
+  }
+  const double least = (double)s.min_p;
+  auto weight = [&](u32 i, float l) {
+    l = x.logit(l);
+    const u32 k = key_of(l);
+    if (!k || !border.keeps(k, i)) {
+      return u64(0);
+    }
+    const double q = x.ratio(l);
+    return q >= least ? (u64)rint(q * x.unit) : u64(0);
+  };
+  draw(a, sh, r, row, weight);
+}
+
+/* The largest logit, or, where only the first token stays or there is none
+ * above -inf, the result: true. */
+__device__ __forceinline__ bool first_only(const SampleArgs &a, int r, const Settings &s,
+                                           float top, u32 first_index) {
+  const bool none = top == -INFINITY;
+  if (!none && !s.first) {
+    return false;
+  }
+  if (threadIdx.x == 0) {
+    a.tokens[r] = none ? -1 : (int)first_index;
+    if (a.logprob) {
+      a.logprob[r] = none ? -INFINITY : 0.0f;
+    }
+  }
+  return true;
+}
+
+template <bool kF32, int kLds>
+__global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
+  __shared__ Shared sh;
+  __shared__ __align__(16) char buffer[std::max(kLds, 16)];
+  const int t = threadIdx.x, r = blockIdx.x;
+  const Row<kF32, kLds> row(a, r, buffer);
+  const Settings s = settings_of(a, r);
+  const float top = block_max(sh, row.take());
+  u32 index = 0xffffffffu;
+  if (s.first) {
+    row.each([&](u32 i, float l) { index = l == top && i < index ? i : index; });
+    for (int o = 32; o; o >>= 1) {
+      const u32 other = (u32)__shfl_xor((int)index, o);
+      index = other < index ? other : index;
+    }
+    if ((t & 63) == 0) {
+      sh.wave_c[t >> 6] = index;
+    }
+    __syncthreads();
+    for (int w = 0; w < kWaves; ++w) {
+      index = sh.wave_c[w] < index ? sh.wave_c[w] : index;
+    }
+  }
+  if (first_only(a, r, s, top, index)) {
+    return;
+  }
+  const Scale x = scale_of(a, s, top);
+  u64 mass = 0;
+  u32 count = 0;
+  if (s.top_k || s.top_p < 1.0f) {
+    sh.mass[t] = 0;
+    sh.count[t] = 0;
+    __syncthreads();
+    row.each([&](u32, float l) {
+      l = x.logit(l);
+      if (l > -INFINITY) {
+        const int b = x.bin(l);
+        atomicAdd(&sh.count[b], 1u);
+        if (!s.top_k) {
+          atomicAdd(&sh.mass[b], x.weight(l));
+        }
+      }
+    });
+    __syncthreads();
+    mass = sh.mass[t];
+    count = sh.count[t];
+    __syncthreads();
+  }
+  finish_bins(a, sh, r, row, s, x, mass, count);
+}
+
+template <bool kF32> void launch(const SampleArgs &a, hipStream_t stream) {
+  const dim3 grid((unsigned)a.rows), block(kThreads);
+  /* the row in LDS where it fits, in two sizes: the smaller leaves room for a
+   * second workgroup on a CU */
+  constexpr int kSize = kF32 ? 4 : 2;
+  if (a.vocab <= 32768 / kSize) {
+    hipLaunchKernelGGL((sample_rows<kF32, 32768>), grid, block, 0, stream, a);
+  } else if (a.vocab <= 131072 / kSize) {
+    hipLaunchKernelGGL((sample_rows<kF32, 131072>), grid, block, 0, stream, a);
+  } else {
+    hipLaunchKernelGGL((sample_rows<kF32, 0>), grid, block, 0, stream, a);
   }
 }
 
 } // namespace
 
 void sample_launch(const SampleArgs &a, hipStream_t stream) {
-  const dim3 grid((unsigned)a.rows);
   if (a.f32) {
-    hipLaunchKernelGGL((sample_rows<true>), grid, dim3(kThreads), 0, stream, a);
+    launch<true>(a, stream);
   } else {
-    hipLaunchKernelGGL((sample_rows<false>), grid, dim3(kThreads), 0, stream, a);
+    launch<false>(a, stream);
   }
   VX_HIP_CHECK(hipGetLastError());
 }
