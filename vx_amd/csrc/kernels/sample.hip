@@ -12,7 +12,7 @@
  *
  * Weights 2^((l - top) c), with c = log2(e) / T and top the largest logit, are
  * taken in 64 bits and kept as 64-bit integers of unit 2^-shift, so many that
- * a row's sum stays within 2^62. Integer sums do not depend on their order:
+ * a row's sum stays within 2^62 (and at most 51). Integer sums do not depend on their order:
  * LDS atomics and any division of the row give the same bits.
  *
  * A first histogram over (top - l) c finds the bin of the border of top-k (by
@@ -43,8 +43,8 @@ constexpr int kWaves = kThreads / 64;
 constexpr int kBins = 1024;      /* one a thread */
 constexpr int kChunk = 4 * kThreads; /* logits of a vector load of every thread */
 constexpr int kList = kThreads;  /* tokens in LDS, one a thread */
-constexpr int kFew = 128;        /* of which one wave handles */
-constexpr float kPerOctave = 16.0f; /* bins per factor of two of the weight: 64 of them in all */
+constexpr int kFew = 256;        /* of them, each compared with each */
+constexpr float kPerOctave = 16.0f; /* bins per factor of two of the weight: 2^64 in all */
 
 /* Rises with l; 0 for -inf (and what counts as it), which is never drawn. */
 __device__ __forceinline__ u32 key_of(float l) {
@@ -54,28 +54,6 @@ __device__ __forceinline__ u32 key_of(float l) {
 }
 __device__ __forceinline__ float logit_of(u32 key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-}
-
-/* 2^d for d <= 0 to 2^-52: 2^(d - k) = e^(ln2 (d - k)) by its Taylor sum to the
- * 12th power (the next term is below 2^-53 at |d - k| = 1/2), times 2^k. */
-__device__ __forceinline__ double exp2_neg(double d) {
-  d = fmax(d, -1000.0);
-  const double k = rint(d);
-  const double x = (d - k) * 0.69314718055994530942;
-  double y = 1.0 / 479001600.0;
-  y = fma(y, x, 1.0 / 39916800.0);
-  y = fma(y, x, 1.0 / 3628800.0);
-  y = fma(y, x, 1.0 / 362880.0);
-  y = fma(y, x, 1.0 / 40320.0);
-  y = fma(y, x, 1.0 / 5040.0);
-  y = fma(y, x, 1.0 / 720.0);
-  y = fma(y, x, 1.0 / 120.0);
-  y = fma(y, x, 1.0 / 24.0);
-  y = fma(y, x, 1.0 / 6.0);
-  y = fma(y, x, 0.5);
-  y = fma(y, x, 1.0);
-  y = fma(y, x, 1.0);
-  return ldexp(y, (int)k);
 }
 
 /* floor(x total) and, with kUp, ceil(x total) of x in (0, 1), exactly: x is 24
@@ -118,33 +96,61 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs &a, int r) {
 }
 
 /* How a row's logits become weights. Where a logit is +inf, those count as 0
- * and the others as -inf. */
+ * and the others as -inf.
+ * 2^d, d <= 0, in units: with k the integer next to 64 d, 2^(k / 64) comes from a
+ * table of 64 powers and the exponent, and 2^(d - k / 64) = e^x, |x| <= ln(2) /
+ * 128, from its Taylor sum to the 5th power: what is left out is below 2^-54. */
 struct Scale {
-  double c, top, unit;
+  double c64, top, unit; /* 64 c */
+  const double *table;   /* 2^(i / 64) units, in LDS */
   float ftop, per;
   bool inf;
 
   __device__ __forceinline__ float logit(float l) const {
     return !inf ? l : l == INFINITY ? 0.0f : -INFINITY;
   }
-  /* of what logit() gives */
-  __device__ __forceinline__ double ratio(float l) const {
-    return exp2_neg(((double)l - top) * c); /* 0 for -inf */
+  /* of what logit() gives, in units, not rounded */
+  __device__ __forceinline__ double units(float l) const {
+    const double d = fmax(((double)l - top) * c64, -8192.0); /* 2^-128: 0 units */
+    const double k = rint(d);
+    const double x = (d - k) * (0.69314718055994530942 / 64.0);
+    double y = fma(x, 1.0 / 120.0, 1.0 / 24.0);
+    y = fma(y, x, 1.0 / 6.0);
+    y = fma(y, x, 0.5);
+    y = fma(y, x, 1.0);
+    y = fma(y, x, 1.0);
+    const int i = (int)k;
+    return ldexp(y * table[i & 63], i >> 6);
   }
-  __device__ __forceinline__ u64 weight(float l) const { return (u64)rint(ratio(l) * unit); }
+  /* to the nearest integer: units stay within 2^51, where adding 2^52 leaves it
+   * in the low bits */
+  static __device__ __forceinline__ u64 whole(double units) {
+    return (u64)__double_as_longlong(units + 0x1p52) & 0xfffffffffffffull;
+  }
+  __device__ __forceinline__ u64 weight(float l) const { return whole(units(l)); }
   /* Falls with l; the last bin's weights are 0. */
   __device__ __forceinline__ int bin(float l) const {
     return (int)fminf(fminf(ftop - l, 3.4028234664e38f) * per, (float)(kBins - 1));
   }
+  /* No logit of a bin up to `b` is lower. */
+  __device__ __forceinline__ float least(int b) const {
+    return per > 0.0f ? ftop - (float)(b + 2) / per : -INFINITY;
+  }
 };
-__device__ __forceinline__ Scale scale_of(const SampleArgs &a, const Settings &s, float top) {
+/* Threads 0 .. 63 fill the table; the caller synchronises. */
+__device__ __forceinline__ Scale scale_of(const SampleArgs &a, const Settings &s, float top,
+                                          double *table) {
   Scale x;
   x.inf = top == INFINITY;
   x.ftop = x.inf ? 0.0f : top;
   x.top = (double)x.ftop;
-  x.c = s.c;
+  x.c64 = s.c * 64.0;
   x.per = s.per;
-  x.unit = ldexp(1.0, 62 - (a.vocab > 1 ? 32 - __clz(a.vocab - 1) : 0));
+  x.unit = ldexp(1.0, min(51, 62 - (a.vocab > 1 ? 32 - __clz(a.vocab - 1) : 0)));
+  x.table = table;
+  if (threadIdx.x < 64) {
+    table[threadIdx.x] = exp2((double)threadIdx.x / 64.0) * x.unit;
+  }
   return x;
 }
 
@@ -179,6 +185,7 @@ struct Shared {
   u32 wave_c[kWaves];
   u32 n;
   Found found;
+  double table[64];
 };
 
 __device__ __forceinline__ u64 block_sum(Shared &sh, u64 v) {
@@ -210,23 +217,28 @@ __device__ __forceinline__ float block_max(Shared &sh, float v) {
 }
 
 /* Which bin a running count or weight over the threads' bins, from thread 0 on,
- * starts at from `above_*` and reaches `want` in; there is one. */
+ * starts at from `above_*` and reaches `want` in; .bin -1 where none does. By
+ * count, weights are not looked at. */
 template <bool kMass>
 __device__ Found find_bin(Shared &sh, u64 mass, u32 count, u64 above_mass, u32 above_count,
                           u64 want) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const u64 ms = wave_scan(mass);
+  const u64 ms = kMass ? wave_scan(mass) : 0;
   const u32 cs = wave_scan(count);
   if (lane == 63) {
     sh.wave_m[wave] = ms;
     sh.wave_c[wave] = cs;
   }
+  if (threadIdx.x == 0) {
+    sh.found.bin = -1;
+  }
   __syncthreads();
-  u64 mb = above_mass + ms - mass;
+  u64 mb = above_mass + ms - (kMass ? mass : 0);
   u32 cb = above_count + cs - count;
-  for (int w = 0; w < wave; ++w) {
-    mb += sh.wave_m[w];
-    cb += sh.wave_c[w];
+#pragma unroll
+  for (int w = 0; w < kWaves - 1; ++w) {
+    mb += kMass && w < wave ? sh.wave_m[w] : 0;
+    cb += w < wave ? sh.wave_c[w] : 0;
   }
   const u64 before = kMass ? mb : cb, own = kMass ? mass : count;
   if (before < want && want <= before + own) {
@@ -325,73 +337,69 @@ __device__ __forceinline__ void put(const SampleArgs &a, int r, int token, u64 w
   }
 }
 
-/* Everything that is left to do for at most kFew tokens in the list, by one
- * wave, two tokens a lane. `mass`: the weight that top_p is a share of, where
- * no top_k is on. */
+/* Everything that is left to do for at most kFew tokens in the list: a token's
+ * place in the order, and the weight before it there and by index, by comparing
+ * it with each, kSlices threads a token. `mass`: the weight that top_p is a
+ * share of, where no top_k is on. */
 __device__ void finish_few(const SampleArgs &a, Shared &sh, int r, const Settings &s,
                            const Scale &x, int n, u64 mass) {
-  const int lane = threadIdx.x;
-  u64 k[2], w[2], before[2] = {0, 0};
-  u32 rank[2] = {0, 0};
-  bool in[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    in[e] = lane + 64 * e < n;
-    k[e] = in[e] ? sh.list_k[lane + 64 * e] : 0;
-    w[e] = in[e] ? sh.list_w[lane + 64 * e] : 0;
+  constexpr int kSlices = kThreads / kFew;
+  const int t = threadIdx.x, e = t % kFew, slice = t / kFew;
+  const bool real = e < n;
+  const u64 k = real ? sh.list_k[e] : 0;
+  const u32 i = ~(u32)k;
+  /* sums over the slices meet in mass[e] and count[e] */
+  if (t < kFew) {
+    sh.mass[t] = 0;
+    sh.count[t] = 0;
+    sh.mass[kFew + t] = 0;
   }
-  for (int j = 0; j < n; ++j) {
-    const u64 kj = sh.list_k[j], wj = sh.list_w[j];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const bool over = kj > k[e];
-      rank[e] += over ? 1u : 0u;
-      before[e] += over ? wj : 0;
+  __syncthreads();
+  if (real) {
+    u64 before = 0;
+    u32 rank = 0;
+#pragma unroll 4
+    for (int j = slice; j < n; j += kSlices) {
+      const bool over = sh.list_k[j] > k;
+      rank += over ? 1u : 0u;
+      before += over ? sh.list_w[j] : 0;
     }
+    atomicAdd(&sh.count[e], rank);
+    atomicAdd(&sh.mass[e], before);
   }
+  __syncthreads();
+  bool in = real;
+  u64 w = real ? sh.list_w[e] : 0;
   if (s.top_k) {
-    mass = 0;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      in[e] = in[e] && rank[e] < (u32)s.top_k;
-      mass += in[e] ? w[e] : 0;
-    }
-    mass = wave_sum64(mass);
+    in = in && sh.count[e] < (u32)s.top_k;
+    mass = s.top_p < 1.0f ? block_sum(sh, in && slice == 0 ? w : 0) : 0;
   }
   if (s.top_p < 1.0f) {
-    const u64 want = part_of<true>(s.top_p, mass);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      in[e] = in[e] && before[e] < want;
-    }
+    in = in && sh.mass[e] < part_of<true>(s.top_p, mass);
   }
-  u64 total = 0;
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (s.min_p > 0.0f) {
-      in[e] = in[e] && x.ratio(logit_of((u32)(k[e] >> 32))) >= (double)s.min_p;
-    }
-    w[e] = in[e] ? w[e] : 0;
-    total += w[e];
-    if (lane + 64 * e < n) {
-      sh.list_w[lane + 64 * e] = w[e];
-    }
+  if (s.min_p > 0.0f) {
+    in = in && x.units(logit_of((u32)(k >> 32))) >= (double)s.min_p * x.unit;
   }
-  total = wave_sum64(total);
+  w = in ? w : 0;
+  const u64 total = block_sum(sh, slice == 0 ? w : 0);
   const u64 target = target_of(a, r, total);
-  u64 upto[2] = {0, 0}; /* over the tokens of lower indexes */
-  for (int j = 0; j < n; ++j) {
-    const u32 ij = ~(u32)sh.list_k[j];
-    const u64 wj = sh.list_w[j];
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      upto[e] += ij < ~(u32)k[e] ? wj : 0;
-    }
+  if (slice == 0 && real) {
+    sh.list_w[e] = w;
   }
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    if (in[e] && upto[e] <= target && target < upto[e] + w[e]) {
-      put(a, r, (int)~(u32)k[e], w[e], total);
+  __syncthreads();
+  if (real) {
+    u64 before = 0;
+#pragma unroll 4
+    for (int j = slice; j < n; j += kSlices) {
+      before += ~(u32)sh.list_k[j] < i ? sh.list_w[j] : 0;
+    }
+    atomicAdd(&sh.mass[kFew + e], before);
+  }
+  __syncthreads();
+  if (in && slice == 0) {
+    const u64 before = sh.mass[kFew + e];
+    if (before <= target && target < before + w) {
+      put(a, r, (int)i, w, total);
     }
   }
 }
@@ -406,8 +414,7 @@ __device__ void finish_list(const SampleArgs &a, Shared &sh, int r, const Settin
   const u32 key = (u32)(kw >> 32), i = ~(u32)kw;
   bool in = mine;
   const u32 hi = key_of(x.ftop);
-  const float least = x.per > 0.0f ? x.ftop - (float)(bin + 2) / x.per : -INFINITY;
-  const u32 lo = max(key_of(least), 1u); /* a bin below the last one's end */
+  const u32 lo = max(key_of(x.least(bin)), 1u);
   auto by_key = [&](auto take) {
     if (in) {
       take(key, [&] { return w; });
@@ -431,7 +438,7 @@ __device__ void finish_list(const SampleArgs &a, Shared &sh, int r, const Settin
     in = in && b.keeps(key, i);
   }
   if (s.min_p > 0.0f) {
-    in = in && x.ratio(logit_of(key)) >= (double)s.min_p;
+    in = in && x.units(logit_of(key)) >= (double)s.min_p * x.unit;
   }
   const u64 total = block_sum(sh, in ? w : 0);
   const u64 target = target_of(a, r, total);
@@ -619,6 +626,45 @@ __device__ void draw(const SampleArgs &a, Shared &sh, int r, const R &row, W wei
   }
 }
 
+/* The row's tokens of bins up to `bin` into the list; how many there are, which
+ * may be more than it holds. */
+template <typename R>
+__device__ int gather(Shared &sh, const R &row, const Scale &x, int bin) {
+  if (threadIdx.x == 0) {
+    sh.n = 0;
+  }
+  __syncthreads();
+  const float least = x.inf ? INFINITY : x.least(bin);
+  row.each([&](u32 i, float l) {
+    if (l >= least) { /* one of a few, mostly */
+      l = x.logit(l);
+      if (l > -INFINITY && x.bin(l) <= bin) {
+        const u32 at = atomicAdd(&sh.n, 1u);
+        if (at < (u32)kList) {
+          sh.list_k[at] = (u64)key_of(l) << 32 | (u32)~i;
+        }
+      }
+    }
+  });
+  __syncthreads();
+  return (int)sh.n;
+}
+
+/* The result from the list's n tokens, those of bins up to `bin`. */
+__device__ void finish(const SampleArgs &a, Shared &sh, int r, const Settings &s, const Scale &x,
+                       int n, u64 mass, int bin) {
+  const int t = threadIdx.x;
+  if (t < n) {
+    sh.list_w[t] = x.weight(logit_of((u32)(sh.list_k[t] >> 32)));
+  }
+  __syncthreads();
+  if (n <= kFew) {
+    finish_few(a, sh, r, s, x, n, mass);
+  } else {
+    finish_list(a, sh, r, s, x, n, mass, bin);
+  }
+}
+
 /* What is left to do once the row's histogram is in the threads' registers
  * (`mass` only where no top_k is on; all of the row's bins). */
 template <typename R>
@@ -628,9 +674,9 @@ __device__ void finish_bins(const SampleArgs &a, Shared &sh, int r, const R &row
   u64 sum = 0;
   Found f;
   if (s.top_k) {
-    /* more than there are above -inf, or into the weights of 0: all of them */
-    const u64 all = block_sum(sh, t == kBins - 1 ? 0 : count);
-    if ((u64)s.top_k > all) {
+    f = find_bin<false>(sh, 0, t == kBins - 1 ? 0 : count, 0, 0, (u64)s.top_k);
+    if (f.bin < 0) {
+      /* more than there are above -inf, or into the weights of 0: all of them */
       s.top_k = 0;
       if (s.top_p < 1.0f) {
         sh.mass[t] = 0;
@@ -644,8 +690,6 @@ __device__ void finish_bins(const SampleArgs &a, Shared &sh, int r, const R &row
         __syncthreads();
         mass = sh.mass[t];
       }
-    } else {
-      f = find_bin<false>(sh, 0, count, 0, 0, (u64)s.top_k);
     }
   }
   if (!s.top_k && s.top_p < 1.0f) {
@@ -654,32 +698,7 @@ __device__ void finish_bins(const SampleArgs &a, Shared &sh, int r, const R &row
   }
   const bool bordered = s.top_k || s.top_p < 1.0f;
   if (bordered && f.above_count + f.count <= (u32)kList) {
-    const int n = (int)(f.above_count + f.count);
-    if (t == 0) {
-      sh.n = 0;
-    }
-    __syncthreads();
-    row.each([&](u32 i, float l) {
-      l = x.logit(l);
-      if (l > -INFINITY && x.bin(l) <= f.bin) {
-        const u32 at = atomicAdd(&sh.n, 1u);
-        sh.list_k[at] = (u64)key_of(l) << 32 | (u32)~i;
-      }
-    });
-    __syncthreads();
-    if (n <= kFew) {
-      if (t < 64) {
-        for (int j = t; j < n; j += 64) {
-          sh.list_w[j] = x.weight(logit_of((u32)(sh.list_k[j] >> 32)));
-        }
-        finish_few(a, sh, r, s, x, n, sum);
-      }
-      return;
-    }
-    if (t < n) {
-      sh.list_w[t] = x.weight(logit_of((u32)(sh.list_k[t] >> 32)));
-    }
-    finish_list(a, sh, r, s, x, n, sum, f.bin);
+    finish(a, sh, r, s, x, gather(sh, row, x, f.bin), sum, f.bin);
     return;
   }
   Border border{0, 0xffffffffu};
@@ -703,8 +722,7 @@ __device__ void finish_bins(const SampleArgs &a, Shared &sh, int r, const R &row
       });
     };
     /* from the top to a bin below the border's */
-    const float per = x.per;
-    const u32 lo = max(per > 0.0f ? key_of(x.ftop - (float)(f.bin + 2) / per) : 0u, 1u);
+    const u32 lo = max(key_of(x.least(f.bin)), 1u);
     const u32 hi = key_of(x.ftop);
     if (s.top_k) {
       const Point p = descend<false>(sh, by_key, lo, hi, 0, 0, (u64)s.top_k);
@@ -720,15 +738,15 @@ __device__ void finish_bins(const SampleArgs &a, Shared &sh, int r, const R &row
       border = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
     }
   }
-  const double least = (double)s.min_p;
+  const double least = (double)s.min_p * x.unit;
   auto weight = [&](u32 i, float l) {
     l = x.logit(l);
     const u32 k = key_of(l);
     if (!k || !border.keeps(k, i)) {
       return u64(0);
     }
-    const double q = x.ratio(l);
-    return q >= least ? (u64)rint(q * x.unit) : u64(0);
+    const double q = x.units(l);
+    return q >= least ? Scale::whole(q) : u64(0);
   };
   draw(a, sh, r, row, weight);
 }
@@ -757,7 +775,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   const int t = threadIdx.x, r = blockIdx.x;
   const Row<kF32, kLds> row(a, r, buffer);
   const Settings s = settings_of(a, r);
-  const float top = block_max(sh, row.take());
+  const float own = row.take();
+  const float top = block_max(sh, own);
   u32 index = 0xffffffffu;
   if (s.first) {
     row.each([&](u32 i, float l) { index = l == top && i < index ? i : index; });
@@ -776,13 +795,32 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   if (first_only(a, r, s, top, index)) {
     return;
   }
-  const Scale x = scale_of(a, s, top);
+  const Scale x = scale_of(a, s, top, sh.table);
   u64 mass = 0;
   u32 count = 0;
   if (s.top_k || s.top_p < 1.0f) {
     sh.mass[t] = 0;
     sh.count[t] = 0;
     __syncthreads();
+    if (s.top_k) {
+      /* The top_k largest lie down to the bin of the top_k-th largest of the
+       * threads' own maxima; mostly there are few more. */
+      const float l = x.logit(own);
+      if (l > -INFINITY) {
+        atomicAdd(&sh.count[x.bin(l)], 1u);
+      }
+      __syncthreads();
+      const Found f = find_bin<false>(sh, 0, sh.count[t], 0, 0, (u64)s.top_k);
+      if (f.bin >= 0 && f.bin < kBins - 1) {
+        const int n = gather(sh, row, x, f.bin);
+        if (n <= kList) {
+          finish(a, sh, r, s, x, n, 0, f.bin);
+          return;
+        }
+      }
+      sh.count[t] = 0;
+      __syncthreads();
+    }
     row.each([&](u32, float l) {
       l = x.logit(l);
       if (l > -INFINITY) {
@@ -796,8 +834,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
     __syncthreads();
     mass = sh.mass[t];
     count = sh.count[t];
-    __syncthreads();
   }
+  __syncthreads();
   finish_bins(a, sh, r, row, s, x, mass, count);
 }
 
