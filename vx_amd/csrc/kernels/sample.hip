@@ -20,9 +20,11 @@
  * bin, mostly a few dozen, then go into LDS and everything else happens there;
  * where they are many, `descend` and the draw go over the row again.
  *
- * sample_rows: a workgroup a row, which it keeps in LDS up to 128 KiB of it. sample_tops and sample_parts: several workgroups a row find its
- * top, then its histogram or weight, in a workspace; the last of a row to
- * finish does the rest.
+ * sample_rows: a workgroup a row, which it keeps in LDS up to 128 KiB of it.
+ * sample_tops, sample_weigh, sample_settle: several workgroups a row, each of a
+ * slice of it, find its top, then its histogram or weight, in a workspace; the
+ * slice that the draw falls in, or the last to leave its few tokens, does the
+ * rest.
  */
 #include "../vx_batch_kernels.h"
 #include "../vx_hip_common.h"
@@ -79,13 +81,16 @@ struct Settings {
   bool first; /* only the first token of the order stays */
   double c;
   float per; /* bins per unit of logit */
+  float u;   /* in [0, 1) */
 };
 __device__ __forceinline__ Settings settings_of(const SampleArgs &a, int r) {
   const float heat = a.temperature ? a.temperature[r] : 1.0f;
   const int top_k = a.top_k ? a.top_k[r] : 0;
   const float top_p = a.top_p ? a.top_p[r] : 1.0f;
   const float min_p = a.min_p ? a.min_p[r] : 0.0f;
+  const float u = a.u[r];
   Settings s;
+  s.u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
   s.first = !(heat > 0.0f) || top_k == 1 || top_p <= 0.0f;
   s.top_k = top_k > 0 && top_k < a.vocab ? top_k : 0;
   s.top_p = top_p < 1.0f ? top_p : 1.0f;
@@ -97,30 +102,39 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs &a, int r) {
 
 /* How a row's logits become weights. Where a logit is +inf, those count as 0
  * and the others as -inf.
- * 2^d, d <= 0, in units: with k the integer next to 64 d, 2^(k / 64) comes from a
- * table of 64 powers and the exponent, and 2^(d - k / 64) = e^x, |x| <= ln(2) /
- * 128, from its Taylor sum to the 5th power: what is left out is below 2^-54. */
+ * 2^d, d <= 0, in units: with k the integer next to d, 2^(d - k) = e^x, |x| <=
+ * ln(2) / 2, by its Taylor sum to the 12th power (what is left out is below
+ * 2^-52), and 2^k by an addition to the exponent. Adding 1.5 * 2^52 to d leaves k
+ * in the low bits: conversions and roundings of 64 bits take four times an
+ * addition's cycles, and a table in LDS twice a longer sum's. */
 struct Scale {
-  double c64, top, unit; /* 64 c */
-  const double *table;   /* 2^(i / 64) units, in LDS */
+  double c, top;
   float ftop, per;
+  int shift; /* a unit is 2^-shift of the largest weight */
   bool inf;
 
-  __device__ __forceinline__ float logit(float l) const {
-    return !inf ? l : l == INFINITY ? 0.0f : -INFINITY;
-  }
-  /* of what logit() gives, in units, not rounded */
+  /* in units, not rounded */
   __device__ __forceinline__ double units(float l) const {
-    const double d = fmax(((double)l - top) * c64, -8192.0); /* 2^-128: 0 units */
-    const double k = rint(d);
-    const double x = (d - k) * (0.69314718055994530942 / 64.0);
-    double y = fma(x, 1.0 / 120.0, 1.0 / 24.0);
-    y = fma(y, x, 1.0 / 6.0);
-    y = fma(y, x, 0.5);
-    y = fma(y, x, 1.0);
-    y = fma(y, x, 1.0);
-    const int i = (int)k;
-    return ldexp(y * table[i & 63], i >> 6);
+    const double d = fmax(((double)l - top) * c, -128.0); /* 0 units */
+    const double t = d + 0x1.8p52;
+    const double f = d - (t - 0x1.8p52);
+    constexpr double ln2 = 0.69314718055994530942;
+    constexpr double q2 = ln2 * ln2, q4 = q2 * q2, q8 = q4 * q4;
+    double y = q8 * q4 / 479001600.0;
+    y = fma(y, f, q8 * q2 * ln2 / 39916800.0);
+    y = fma(y, f, q8 * q2 / 3628800.0);
+    y = fma(y, f, q8 * ln2 / 362880.0);
+    y = fma(y, f, q8 / 40320.0);
+    y = fma(y, f, q4 * q2 * ln2 / 5040.0);
+    y = fma(y, f, q4 * q2 / 720.0);
+    y = fma(y, f, q4 * ln2 / 120.0);
+    y = fma(y, f, q4 / 24.0);
+    y = fma(y, f, q2 * ln2 / 6.0);
+    y = fma(y, f, q2 / 2.0);
+    y = fma(y, f, ln2);
+    y = fma(y, f, 1.0);
+    const int k = (int)(u32)__double_as_longlong(t) + shift;
+    return __hiloint2double(__double2hiint(y) + (k << 20), __double2loint(y));
   }
   /* to the nearest integer: units stay within 2^51, where adding 2^52 leaves it
    * in the low bits */
@@ -128,6 +142,8 @@ struct Scale {
     return (u64)__double_as_longlong(units + 0x1p52) & 0xfffffffffffffull;
   }
   __device__ __forceinline__ u64 weight(float l) const { return whole(units(l)); }
+  /* `min_p` in units. */
+  __device__ __forceinline__ double share(float min_p) const { return ldexp((double)min_p, shift); }
   /* Falls with l; the last bin's weights are 0. */
   __device__ __forceinline__ int bin(float l) const {
     return (int)fminf(fminf(ftop - l, 3.4028234664e38f) * per, (float)(kBins - 1));
@@ -137,37 +153,50 @@ struct Scale {
     return per > 0.0f ? ftop - (float)(b + 2) / per : -INFINITY;
   }
 };
-/* Threads 0 .. 63 fill the table; the caller synchronises. */
-__device__ __forceinline__ Scale scale_of(const SampleArgs &a, const Settings &s, float top,
-                                          double *table) {
+__device__ __forceinline__ Scale scale_of(const SampleArgs &a, const Settings &s, float top) {
   Scale x;
   x.inf = top == INFINITY;
   x.ftop = x.inf ? 0.0f : top;
   x.top = (double)x.ftop;
-  x.c64 = s.c * 64.0;
+  x.c = s.c;
   x.per = s.per;
-  x.unit = ldexp(1.0, min(51, 62 - (a.vocab > 1 ? 32 - __clz(a.vocab - 1) : 0)));
-  x.table = table;
-  if (threadIdx.x < 64) {
-    table[threadIdx.x] = exp2((double)threadIdx.x / 64.0) * x.unit;
-  }
+  x.shift = min(51, 62 - (a.vocab > 1 ? 32 - __clz(a.vocab - 1) : 0));
   return x;
 }
 
-__device__ __forceinline__ u64 wave_sum64(u64 v) {
-  for (int o = 32; o; o >>= 1) {
-    v += __shfl_xor(v, o);
-  }
+/* A value of another lane by VALU data movement; 0 where there is none. */
+template <int kCtrl, int kRows> __device__ __forceinline__ u32 dpp(u32 v) {
+  return (u32)__builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xf, false);
+}
+template <int kCtrl, int kRows> __device__ __forceinline__ u64 dpp(u64 v) {
+  return (u64)dpp<kCtrl, kRows>((u32)(v >> 32)) << 32 | dpp<kCtrl, kRows>((u32)v);
+}
+/* Inclusive sum over the wave's lanes up to this one: within rows of 16 lanes by
+ * shifts of 1, 2, 4 and 8, then the last lanes of rows and of halves. */
+template <typename T> __device__ __forceinline__ T wave_scan(T v) {
+  v += dpp<0x111, 0xf>(v);
+  v += dpp<0x112, 0xf>(v);
+  v += dpp<0x114, 0xf>(v);
+  v += dpp<0x118, 0xf>(v);
+  v += dpp<0x142, 0xa>(v); /* lane 15 of rows 0 and 2 to the next row */
+  v += dpp<0x143, 0xc>(v); /* lane 31 to rows 2 and 3 */
   return v;
 }
-/* Inclusive, over the wave's lanes up to this one. */
-template <typename T> __device__ __forceinline__ T wave_scan(T v) {
-  const int lane = threadIdx.x & 63;
-  for (int o = 1; o < 64; o <<= 1) {
-    const T w = __shfl_up(v, o);
-    v += lane >= o ? w : 0;
-  }
-  return v;
+__device__ __forceinline__ u64 lane63(u64 v) {
+  return (u64)(u32)__builtin_amdgcn_readlane((int)(u32)(v >> 32), 63) << 32 |
+         (u32)__builtin_amdgcn_readlane((int)(u32)v, 63);
+}
+__device__ __forceinline__ u64 wave_sum64(u64 v) { return lane63(wave_scan(v)); }
+/* The wave's largest, of values above 0 or 0. */
+__device__ __forceinline__ u64 wave_max64(u64 v) {
+  auto up = [&](u64 w) { v = w > v ? w : v; };
+  up(dpp<0x111, 0xf>(v));
+  up(dpp<0x112, 0xf>(v));
+  up(dpp<0x114, 0xf>(v));
+  up(dpp<0x118, 0xf>(v));
+  up(dpp<0x142, 0xa>(v));
+  up(dpp<0x143, 0xc>(v));
+  return lane63(v);
 }
 
 struct Found {
@@ -176,6 +205,12 @@ struct Found {
   int bin;
 };
 
+/* Which thread's `own` the draw falls in, by rising thread; with the row's weight,
+ * and where in that part it does. */
+struct Drawn {
+  u64 total, target;
+  int at;
+};
 struct Shared {
   u64 mass[kBins];
   u64 list_w[kList];
@@ -185,7 +220,7 @@ struct Shared {
   u32 wave_c[kWaves];
   u32 n;
   Found found;
-  double table[64];
+  Drawn drawn;
 };
 
 __device__ __forceinline__ u64 block_sum(Shared &sh, u64 v) {
@@ -220,7 +255,7 @@ __device__ __forceinline__ float block_max(Shared &sh, float v) {
  * starts at from `above_*` and reaches `want` in; .bin -1 where none does. By
  * count, weights are not looked at. */
 template <bool kMass>
-__device__ Found find_bin(Shared &sh, u64 mass, u32 count, u64 above_mass, u32 above_count,
+__device__ __forceinline__ Found find_bin(Shared &sh, u64 mass, u32 count, u64 above_mass, u32 above_count,
                           u64 want) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const u64 ms = kMass ? wave_scan(mass) : 0;
@@ -259,7 +294,7 @@ struct Point {
   Found f;
 };
 template <bool kMass, typename Each>
-__device__ Point descend(Shared &sh, Each each, u32 lo, u32 hi, u64 above_mass, u32 above_count,
+__device__ __forceinline__ Point descend(Shared &sh, Each each, u32 lo, u32 hi, u64 above_mass, u32 above_count,
                          u64 want) {
   const int t = threadIdx.x;
   for (;;) {
@@ -301,7 +336,7 @@ struct Border {
 
 /* The border at `point`, whose first `ties` tokens stay. */
 template <typename Each>
-__device__ Border border_at(Shared &sh, Each each, const Point &point, u64 ties, int vocab) {
+__device__ __forceinline__ Border border_at(Shared &sh, Each each, const Point &point, u64 ties, int vocab) {
   if (ties >= point.f.count) {
     return Border{point.key, 0xffffffffu};
   }
@@ -325,9 +360,28 @@ __device__ __forceinline__ u64 ties_of(const Found &f, u64 want) {
   return (want - f.above_mass + each - 1) / each;
 }
 
-__device__ __forceinline__ u64 target_of(const SampleArgs &a, int r, u64 total) {
-  const float u = a.u[r];
-  return part_of<false>(u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f, total);
+__device__ __forceinline__ Drawn draw_part(Shared &sh, u64 own, float u) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const u64 upto = wave_scan(own);
+  if (lane == 63) {
+    sh.wave_m[wave] = upto;
+  }
+  __syncthreads();
+  u64 total = 0, before = upto - own;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const u64 m = sh.wave_m[w];
+    total += m;
+    before += w < wave ? m : 0;
+  }
+  const u64 target = part_of<false>(u, total);
+  if (before <= target && target < before + own) {
+    sh.drawn = Drawn{total, target - before, (int)threadIdx.x};
+  }
+  __syncthreads();
+  const Drawn d = sh.drawn;
+  __syncthreads();
+  return d;
 }
 
 __device__ __forceinline__ void put(const SampleArgs &a, int r, int token, u64 w, u64 total) {
@@ -341,7 +395,7 @@ __device__ __forceinline__ void put(const SampleArgs &a, int r, int token, u64 w
  * place in the order, and the weight before it there and by index, by comparing
  * it with each, kSlices threads a token. `mass`: the weight that top_p is a
  * share of, where no top_k is on. */
-__device__ void finish_few(const SampleArgs &a, Shared &sh, int r, const Settings &s,
+__device__ __forceinline__ void finish_few(const SampleArgs &a, Shared &sh, int r, const Settings &s,
                            const Scale &x, int n, u64 mass) {
   constexpr int kSlices = kThreads / kFew;
   const int t = threadIdx.x, e = t % kFew, slice = t / kFew;
@@ -378,11 +432,11 @@ __device__ void finish_few(const SampleArgs &a, Shared &sh, int r, const Setting
     in = in && sh.mass[e] < part_of<true>(s.top_p, mass);
   }
   if (s.min_p > 0.0f) {
-    in = in && x.units(logit_of((u32)(k >> 32))) >= (double)s.min_p * x.unit;
+    in = in && x.units(logit_of((u32)(k >> 32))) >= x.share(s.min_p);
   }
   w = in ? w : 0;
   const u64 total = block_sum(sh, slice == 0 ? w : 0);
-  const u64 target = target_of(a, r, total);
+  const u64 target = part_of<false>(s.u, total);
   if (slice == 0 && real) {
     sh.list_w[e] = w;
   }
@@ -405,7 +459,7 @@ __device__ void finish_few(const SampleArgs &a, Shared &sh, int r, const Setting
 }
 
 /* The same for up to kList tokens, one a thread, of bins up to `bin`. */
-__device__ void finish_list(const SampleArgs &a, Shared &sh, int r, const Settings &s,
+__device__ __forceinline__ void finish_list(const SampleArgs &a, Shared &sh, int r, const Settings &s,
                             const Scale &x, int n, u64 mass, int bin) {
   const int t = threadIdx.x;
   const bool mine = t < n;
@@ -438,10 +492,10 @@ __device__ void finish_list(const SampleArgs &a, Shared &sh, int r, const Settin
     in = in && b.keeps(key, i);
   }
   if (s.min_p > 0.0f) {
-    in = in && x.units(logit_of(key)) >= (double)s.min_p * x.unit;
+    in = in && x.units(logit_of(key)) >= x.share(s.min_p);
   }
   const u64 total = block_sum(sh, in ? w : 0);
-  const u64 target = target_of(a, r, total);
+  const u64 target = part_of<false>(s.u, total);
   const Point p = descend<true>(
       sh,
       [&](auto take) {
@@ -474,19 +528,21 @@ template <bool kF32, int kLds> struct Row {
   typedef typename Four<kF32>::whole VA;
   static constexpr int kSize = kF32 ? 4 : 2;
   const char *p;
-  int vocab;
-  u32 lds; /* where LDS holds it */
+  int begin, end; /* the part of it that is meant */
+  u32 lds;        /* where LDS holds it (from index 0 on) */
+  bool inf;       /* it holds +inf: those are 0, the others -inf */
 
   __device__ __forceinline__ Row(const SampleArgs &a, int r, const char *buffer)
-      : p(static_cast<const char *>(a.logits) + (int64_t)r * a.stride * kSize), vocab(a.vocab),
-        lds(kLds ? (u32)(uintptr_t)(const VX_LDS char *)buffer : 0u) {}
+      : p(static_cast<const char *>(a.logits) + (int64_t)r * a.stride * kSize), begin(0),
+        end(a.vocab), lds(kLds ? (u32)(uintptr_t)(const VX_LDS char *)buffer : 0u),
+        inf(false) {}
 
   static __device__ __forceinline__ float clean(float l) {
     return l > -INFINITY ? l + 0.0f : -INFINITY;
   }
-  __device__ __forceinline__ void from_memory(int64_t i, int64_t end, float (&l)[4]) const {
+  __device__ __forceinline__ void from_memory(int i, int end, float (&l)[4]) const {
     if (i + 3 < end) {
-      const V v = *reinterpret_cast<const V *>(p + i * kSize);
+      const V v = *reinterpret_cast<const V *>(p + (int64_t)i * kSize);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         l[e] = clean(Four<kF32>::value(v[e]));
@@ -505,8 +561,21 @@ template <bool kF32, int kLds> struct Row {
       }
     }
   }
-  __device__ __forceinline__ void load4(int64_t i, int64_t end, float (&l)[4]) const {
+  __device__ __forceinline__ void load4(int i, int end, float (&l)[4]) const {
+    load(i, end, l);
+    if (inf) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        l[e] = l[e] == INFINITY ? 0.0f : -INFINITY;
+      }
+    }
+  }
+  __device__ __forceinline__ void load(int i, int end, float (&l)[4]) const {
     if constexpr (kLds > 0) {
+      if (i >= end) {
+        l[0] = l[1] = l[2] = l[3] = -INFINITY;
+        return;
+      }
       const VA v = *(const VX_LDS VA *)(uintptr_t)(lds + (u32)i * kSize);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -516,13 +585,13 @@ template <bool kF32, int kLds> struct Row {
       from_memory(i, end, l);
     }
   }
-  /* The row's first reading: its largest logit, and into LDS. */
+  /* The first reading: the thread's largest logit, and into LDS. */
   __device__ __forceinline__ float take() const {
     float top = -INFINITY;
 #pragma unroll 4
-    for (int64_t i = 4 * threadIdx.x; i < vocab; i += kChunk) {
+    for (int i = begin + 4 * threadIdx.x; i < end; i += kChunk) {
       float l[4];
-      from_memory(i, vocab, l);
+      from_memory(i, end, l);
       VA v;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -539,39 +608,55 @@ template <bool kF32, int kLds> struct Row {
     }
     return top;
   }
-  /* f(index, logit), in no order. */
+  /* f(index, logit), in no order. Out of memory four loads a thread are in
+   * flight, -inf past the end. */
   template <typename F> __device__ __forceinline__ void each(F f) const {
+    constexpr int kAhead = kLds > 0 ? 1 : 4;
 #pragma unroll 1
-    for (int64_t i = 4 * threadIdx.x; i < vocab; i += kChunk) {
-      float v[4];
-      load4(i, vocab, v);
+    for (int i = begin + 4 * threadIdx.x; i < end; i += kAhead * kChunk) {
+      float v[kAhead][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        f((u32)i + e, v[e]);
+      for (int j = 0; j < kAhead; ++j) {
+        load4(i + j * kChunk, end, v[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f((u32)(i + j * kChunk + e), v[j][e]);
+        }
       }
     }
   }
 };
 
-/* The draw over a row, `weight` giving a token's (0 if it does not stay). The
- * row, then the part of it that the sum falls in, is cut into a part for each
- * wave until it is a chunk. */
+/* The draw over a row's part, `weight` giving a token's (0 if it does not stay);
+ * with `total`, the weight of the whole row, of the token in which the part's
+ * sum passes `target`. The part, then the part of it that the sum falls in, is
+ * cut into one for each wave until it is a chunk. */
 template <typename R, typename W>
-__device__ void draw(const SampleArgs &a, Shared &sh, int r, const R &row, W weight) {
+__device__ __forceinline__ void draw(const SampleArgs &a, Shared &sh, int r, const R &row, float u, W weight,
+                     u64 total = 0, u64 target = 0) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  int64_t begin = 0, end = row.vocab;
-  u64 total = 0, target = 0;
+  int begin = row.begin, end = row.end;
   while (end - begin > kChunk) {
-    const int64_t per = ((end - begin + kWaves - 1) / kWaves + 3) / 4 * 4;
-    const int64_t i0 = begin + wave * per, i1 = i0 + per < end ? i0 + per : end;
+    const int per = ((end - begin + kWaves - 1) / kWaves + 3) / 4 * 4;
+    const int i0 = min(begin + wave * per, end), i1 = min(i0 + per, end);
     u64 sum = 0;
+    constexpr int kAhead = 4;
 #pragma unroll 1
-    for (int64_t i = i0 + 4 * lane; i < i1; i += 256) {
-      float v[4];
-      row.load4(i, i1, v);
+    for (int i = i0 + 4 * lane; i < i1; i += kAhead * 256) {
+      float v[kAhead][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sum += weight((u32)(i + e), v[e]);
+      for (int j = 0; j < kAhead; ++j) {
+        row.load4(i + j * 256, i1, v[j]);
+      }
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sum += weight((u32)(i + j * 256 + e), v[j][e]);
+        }
       }
     }
     sum = wave_sum64(sum);
@@ -579,24 +664,33 @@ __device__ void draw(const SampleArgs &a, Shared &sh, int r, const R &row, W wei
       sh.wave_m[wave] = sum;
     }
     __syncthreads();
-    if (total == 0) {
+    u64 part[kWaves];
+    u64 all = 0;
 #pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        total += sh.wave_m[w];
-      }
-      target = target_of(a, r, total);
+    for (int w = 0; w < kWaves; ++w) {
+      part[w] = sh.wave_m[w];
+      all += part[w];
+    }
+    if (total == 0) {
+      total = all;
+      target = part_of<false>(u, total);
     }
     int at = 0;
-    for (; at + 1 < kWaves && target >= sh.wave_m[at]; ++at) {
-      target -= sh.wave_m[at];
+    u64 before = 0, run = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      run += part[w];
+      at = target >= run ? w + 1 : at;
+      before = target >= run ? run : before;
     }
+    target -= before;
     __syncthreads();
     begin += at * per;
-    end = begin + per < end ? begin + per : end;
+    end = min(begin + per, end);
   }
   float v[4];
   u64 w[4], sum = 0;
-  const int64_t i = begin + 4 * t;
+  const int i = begin + 4 * t;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
     v[e] = -INFINITY;
@@ -609,16 +703,22 @@ __device__ void draw(const SampleArgs &a, Shared &sh, int r, const R &row, W wei
     w[e] = weight((u32)(i + e), v[e]);
     sum += w[e];
   }
+  int at;
   if (total == 0) {
-    total = block_sum(sh, sum);
-    target = target_of(a, r, total);
-  }
-  const Found f = find_bin<true>(sh, sum, 0, 0, 0, target + 1);
-  if (f.bin == t) {
+    const Drawn d = draw_part(sh, sum, u);
+    total = d.total;
+    target = d.target;
+    at = d.at;
+  } else {
+    const Found f = find_bin<true>(sh, sum, 0, 0, 0, target + 1);
     target -= f.above_mass;
+    at = f.bin;
+  }
+  if (at == t) {
+#pragma unroll
     for (int e = 0; e < 4; ++e) {
       if (target < w[e]) {
-        put(a, r, (int)(i + e), w[e], total);
+        put(a, r, i + e, w[e], total);
         return;
       }
       target -= w[e];
@@ -626,22 +726,23 @@ __device__ void draw(const SampleArgs &a, Shared &sh, int r, const R &row, W wei
   }
 }
 
-/* The row's tokens of bins up to `bin` into the list; how many there are, which
- * may be more than it holds. */
-template <typename R>
-__device__ int gather(Shared &sh, const R &row, const Scale &x, int bin) {
+/* The row's tokens of bins up to `bin` (kOne: of that bin) into the list; how
+ * many there are, of which it holds the first kCap. */
+template <bool kOne = false, int kCap, typename R>
+__device__ __forceinline__ int gather(Shared &sh, const R &row, const Scale &x, int bin,
+                                      u64 (&list)[kCap]) {
   if (threadIdx.x == 0) {
     sh.n = 0;
   }
   __syncthreads();
-  const float least = x.inf ? INFINITY : x.least(bin);
+  const float least = x.least(bin);
   row.each([&](u32 i, float l) {
     if (l >= least) { /* one of a few, mostly */
-      l = x.logit(l);
-      if (l > -INFINITY && x.bin(l) <= bin) {
+      const int b = x.bin(l);
+      if (l > -INFINITY && (kOne ? b == bin : b <= bin)) {
         const u32 at = atomicAdd(&sh.n, 1u);
-        if (at < (u32)kList) {
-          sh.list_k[at] = (u64)key_of(l) << 32 | (u32)~i;
+        if (at < (u32)kCap) {
+          list[at] = (u64)key_of(l) << 32 | (u32)~i;
         }
       }
     }
@@ -651,7 +752,7 @@ __device__ int gather(Shared &sh, const R &row, const Scale &x, int bin) {
 }
 
 /* The result from the list's n tokens, those of bins up to `bin`. */
-__device__ void finish(const SampleArgs &a, Shared &sh, int r, const Settings &s, const Scale &x,
+__device__ __forceinline__ void finish(const SampleArgs &a, Shared &sh, int r, const Settings &s, const Scale &x,
                        int n, u64 mass, int bin) {
   const int t = threadIdx.x;
   if (t < n) {
@@ -665,90 +766,129 @@ __device__ void finish(const SampleArgs &a, Shared &sh, int r, const Settings &s
   }
 }
 
-/* What is left to do once the row's histogram is in the threads' registers
- * (`mass` only where no top_k is on; all of the row's bins). */
+/* A token's weight, where min_p and (kBordered) a border keep it, else 0. */
+template <bool kBordered> struct Keep {
+  const Scale &x;
+  double least; /* units */
+  Border border;
+
+  __device__ __forceinline__ u64 operator()(u32 i, float l) const {
+    const double q = x.units(l);
+    const u64 w = q >= least ? Scale::whole(q) : u64(0);
+    return !kBordered || border.keeps(key_of(l), i) ? w : u64(0);
+  }
+};
+
+/* Where the border of top_k, or without it of top_p, lies in the row's histogram,
+ * which is in the threads' registers (`mass` only where no top_k is on). */
+struct Where {
+  Found f;
+  u64 sum; /* the row's weight, without top_k */
+  int bin; /* the tokens of bins up to this one are enough to go on with */
+  u32 n;   /* so many */
+};
+/* .f.bin -1: top_k is more than there are above -inf, or reaches the weights of
+ * 0, so that it hides nothing. */
+__device__ __forceinline__ Where locate(Shared &sh, const Settings &s, u64 mass, u32 count) {
+  const int t = threadIdx.x;
+  Where w;
+  w.sum = 0;
+  if (s.top_k) {
+    w.f = find_bin<false>(sh, 0, t == kBins - 1 ? 0 : count, 0, 0, (u64)s.top_k);
+  } else {
+    w.sum = block_sum(sh, mass);
+    w.f = find_bin<true>(sh, mass, count, 0, 0, part_of<true>(s.top_p, w.sum));
+  }
+  w.bin = w.f.bin;
+  w.n = w.f.above_count + w.f.count;
+  if (s.min_p > 0.0f && (!s.top_k || s.top_p >= 1.0f)) {
+    /* weights from min_p on lie down to here; nothing below is needed unless
+     * top_p is a share of what top_k keeps */
+    const int bin = (int)fminf(-log2f(s.min_p) * kPerOctave + 2.0f, (float)(kBins - 2));
+    if (bin < w.bin) {
+      w.bin = bin;
+      w.n = (u32)block_sum(sh, t <= bin ? count : 0);
+    }
+  }
+  return w;
+}
+
+/* What is left to do once the row's histogram is known. */
 template <typename R>
-__device__ void finish_bins(const SampleArgs &a, Shared &sh, int r, const R &row, Settings s,
+__device__ __forceinline__ void finish_bins(const SampleArgs &a, Shared &sh, int r, const R &row, Settings s,
                             const Scale &x, u64 mass, u32 count) {
   const int t = threadIdx.x;
-  u64 sum = 0;
-  Found f;
-  if (s.top_k) {
-    f = find_bin<false>(sh, 0, t == kBins - 1 ? 0 : count, 0, 0, (u64)s.top_k);
-    if (f.bin < 0) {
-      /* more than there are above -inf, or into the weights of 0: all of them */
+  Where at;
+  bool bordered = s.top_k || s.top_p < 1.0f;
+  if (bordered) {
+    at = locate(sh, s, mass, count);
+    if (at.f.bin < 0) {
       s.top_k = 0;
-      if (s.top_p < 1.0f) {
+      bordered = s.top_p < 1.0f;
+      if (bordered) {
         sh.mass[t] = 0;
         __syncthreads();
         row.each([&](u32, float l) {
-          l = x.logit(l);
-          if (l > -INFINITY) {
+            if (l > -INFINITY) {
             atomicAdd(&sh.mass[x.bin(l)], x.weight(l));
           }
         });
         __syncthreads();
-        mass = sh.mass[t];
+        at = locate(sh, s, sh.mass[t], count);
       }
     }
   }
-  if (!s.top_k && s.top_p < 1.0f) {
-    sum = block_sum(sh, mass);
-    f = find_bin<true>(sh, mass, count, 0, 0, part_of<true>(s.top_p, sum));
-  }
-  const bool bordered = s.top_k || s.top_p < 1.0f;
-  if (bordered && f.above_count + f.count <= (u32)kList) {
-    finish(a, sh, r, s, x, gather(sh, row, x, f.bin), sum, f.bin);
+  if (bordered && at.n <= (u32)kList) {
+    finish(a, sh, r, s, x, gather(sh, row, x, at.bin, sh.list_k), at.sum, at.bin);
     return;
   }
-  Border border{0, 0xffffffffu};
-  if (bordered) {
+  if (!bordered) {
+    draw(a, sh, r, row, s.u, Keep<false>{x, x.share(s.min_p), {}});
+    return;
+  }
+  Keep<true> keep{x, x.share(s.min_p), {0, 0xffffffffu}};
+  {
+    /* the border's own bin, then, after top_k, what that keeps */
+    bool all = false;
+    auto passes = [&](u32 k, u32 i, float l) {
+      return all ? k && keep.border.keeps(k, i) : k && x.bin(l) == at.f.bin;
+    };
     auto by_key = [&](auto take) {
       row.each([&](u32 i, float l) {
-        l = x.logit(l);
         const u32 k = key_of(l);
-        if (k && border.keeps(k, i)) {
+        if (passes(k, i, l)) {
           take(k, [&] { return x.weight(l); });
         }
       });
     };
     auto both = [&](auto take) {
       row.each([&](u32 i, float l) {
-        l = x.logit(l);
         const u32 k = key_of(l);
-        if (k && border.keeps(k, i)) {
+        if (passes(k, i, l)) {
           take(k, i, [&] { return x.weight(l); });
         }
       });
     };
-    /* from the top to a bin below the border's */
-    const u32 lo = max(key_of(x.least(f.bin)), 1u);
-    const u32 hi = key_of(x.ftop);
+    const u32 lo = max(key_of(x.least(at.f.bin)), 1u), hi = key_of(x.ftop);
     if (s.top_k) {
-      const Point p = descend<false>(sh, by_key, lo, hi, 0, 0, (u64)s.top_k);
-      border = border_at(sh, both, p, (u64)s.top_k - p.f.above_count, a.vocab);
+      const Point p =
+          descend<false>(sh, by_key, lo, hi, 0, at.f.above_count, (u64)s.top_k);
+      keep.border = border_at(sh, both, p, (u64)s.top_k - p.f.above_count, a.vocab);
       if (s.top_p < 1.0f) {
-        by_key([&](u32, auto weight) { sum += weight(); });
-        sum = block_sum(sh, sum);
+        all = true;
+        at.sum = 0;
+        by_key([&](u32, auto weight) { at.sum += weight(); });
+        at.sum = block_sum(sh, at.sum);
+        at.f.above_mass = 0;
       }
     }
     if (s.top_p < 1.0f) {
-      const u64 want = part_of<true>(s.top_p, sum);
-      const Point p = descend<true>(sh, by_key, lo, hi, 0, 0, want);
-      border = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
+      const u64 want = part_of<true>(s.top_p, at.sum);
+      const Point p = descend<true>(sh, by_key, lo, hi, at.f.above_mass, 0, want);
+      keep.border = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
     }
   }
-  const double least = (double)s.min_p * x.unit;
-  auto weight = [&](u32 i, float l) {
-    l = x.logit(l);
-    const u32 k = key_of(l);
-    if (!k || !border.keeps(k, i)) {
-      return u64(0);
-    }
-    const double q = x.units(l);
-    return q >= least ? Scale::whole(q) : u64(0);
-  };
-  draw(a, sh, r, row, weight);
+  draw(a, sh, r, row, s.u, keep);
 }
 
 /* The largest logit, or, where only the first token stays or there is none
@@ -773,7 +913,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   __shared__ Shared sh;
   __shared__ __align__(16) char buffer[std::max(kLds, 16)];
   const int t = threadIdx.x, r = blockIdx.x;
-  const Row<kF32, kLds> row(a, r, buffer);
+  Row<kF32, kLds> row(a, r, buffer);
   const Settings s = settings_of(a, r);
   const float own = row.take();
   const float top = block_max(sh, own);
@@ -795,7 +935,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   if (first_only(a, r, s, top, index)) {
     return;
   }
-  const Scale x = scale_of(a, s, top, sh.table);
+  const Scale x = scale_of(a, s, top);
+  row.inf = x.inf;
   u64 mass = 0;
   u32 count = 0;
   if (s.top_k || s.top_p < 1.0f) {
@@ -805,14 +946,14 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
     if (s.top_k) {
       /* The top_k largest lie down to the bin of the top_k-th largest of the
        * threads' own maxima; mostly there are few more. */
-      const float l = x.logit(own);
+      const float l = !x.inf ? own : own == INFINITY ? 0.0f : -INFINITY;
       if (l > -INFINITY) {
         atomicAdd(&sh.count[x.bin(l)], 1u);
       }
       __syncthreads();
       const Found f = find_bin<false>(sh, 0, sh.count[t], 0, 0, (u64)s.top_k);
       if (f.bin >= 0 && f.bin < kBins - 1) {
-        const int n = gather(sh, row, x, f.bin);
+        const int n = gather(sh, row, x, f.bin, sh.list_k);
         if (n <= kList) {
           finish(a, sh, r, s, x, n, 0, f.bin);
           return;
@@ -822,7 +963,6 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
       __syncthreads();
     }
     row.each([&](u32, float l) {
-      l = x.logit(l);
       if (l > -INFINITY) {
         const int b = x.bin(l);
         atomicAdd(&sh.count[b], 1u);
@@ -839,8 +979,275 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
   finish_bins(a, sh, r, row, s, x, mass, count);
 }
 
-template <bool kF32> void launch(const SampleArgs &a, hipStream_t stream) {
+/* ---- several workgroups a row ---- */
+
+/* Tokens of one bin that are settled in LDS: at 16 bins per factor of two, a
+ * bell of 131072 logits two units wide has up to 1100 in one. */
+constexpr int kBinList = 4096;
+
+/* A row's workspace, and after it for each slice its first token, its weight,
+ * and (where top_p alone makes the border) its bins' weights. */
+struct Shelf {
+  u64 mass[kBins];
+  u64 list[kBinList];
+  u32 count[kBins];
+  u32 n, ticket;
+
+  __device__ __forceinline__ u64 *tops() { return reinterpret_cast<u64 *>(this + 1); }
+  __device__ __forceinline__ u64 *sums(int slices) { return tops() + slices; }
+  __device__ __forceinline__ u64 *bins(int slices, int slice) {
+    return sums(slices) + slices + (int64_t)slice * kBins;
+  }
+};
+static_assert(sizeof(Shelf) % 8 == 0, "what follows is of 64-bit words");
+
+struct Split {
+  int slices, slice; /* and logits of one */
+  char *ws;
+  int64_t shelf; /* bytes from one row's to the next */
+};
+
+__device__ __forceinline__ u64 load_far(const u64 *p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ void store_far(u64 *p, u64 v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
+/* A slice's first token (its key, then the index's complement). */
+template <bool kF32> __global__ __launch_bounds__(kThreads) void sample_tops(SampleArgs a, Split p) {
+  __shared__ u64 wave_best[kWaves];
+  const int t = threadIdx.x, r = blockIdx.x % a.rows, slice = blockIdx.x / a.rows;
+  Row<kF32, 0> row(a, r, nullptr);
+  row.begin = slice * p.slice;
+  row.end = min(row.begin + p.slice, a.vocab);
+  float top = -INFINITY;
+  u32 at = 0;
+  row.each([&](u32 i, float l) { /* indexes rise: the first of equals stays */
+    at = l > top ? i : at;
+    top = fmaxf(top, l);
+  });
+  const u32 k = key_of(top);
+  u64 best = wave_max64(k ? (u64)k << 32 | (u32)~at : 0);
+  if ((t & 63) == 0) {
+    wave_best[t >> 6] = best;
+  }
+  __syncthreads();
+  Shelf *shelf = reinterpret_cast<Shelf *>(p.ws + r * p.shelf);
+  if (t == 0) {
+    for (int w = 1; w < kWaves; ++w) {
+      best = wave_best[w] > best ? wave_best[w] : best;
+    }
+    shelf->tops()[slice] = best;
+  }
+  if (slice == 0) {
+    shelf->mass[t] = 0;
+    shelf->count[t] = 0;
+    if (t == 0) {
+      shelf->n = 0;
+      shelf->ticket = 0;
+    }
+  }
+}
+
+/* The row's first token, from its slices'. */
+__device__ __forceinline__ u64 first_of(Shared &sh, Shelf *shelf, int slices) {
+  const int t = threadIdx.x;
+  u64 best = wave_max64(t < slices ? shelf->tops()[t] : 0);
+  if ((t & 63) == 0) {
+    sh.wave_m[t >> 6] = best;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    best = sh.wave_m[w] > best ? sh.wave_m[w] : best;
+  }
+  __syncthreads();
+  return best;
+}
+
+/* A slice's weight, or its part of the row's histogram. */
+template <bool kF32> __global__ __launch_bounds__(kThreads) void sample_weigh(SampleArgs a, Split p) {
+  __shared__ Shared sh;
+  const int t = threadIdx.x, r = blockIdx.x % a.rows, slice = blockIdx.x / a.rows;
+  Shelf *shelf = reinterpret_cast<Shelf *>(p.ws + r * p.shelf);
+  const Settings s = settings_of(a, r);
+  const u64 first = first_of(sh, shelf, p.slices);
+  if (!first || s.first) {
+    return;
+  }
+  const Scale x = scale_of(a, s, logit_of((u32)(first >> 32)));
+  Row<kF32, 0> row(a, r, nullptr);
+  row.inf = x.inf;
+  row.begin = slice * p.slice;
+  row.end = min(row.begin + p.slice, a.vocab);
+  sh.mass[t] = 0;
+  sh.count[t] = 0;
+  __syncthreads();
+  if (!s.top_k && s.top_p >= 1.0f) {
+    const Keep<false> keep{x, x.share(s.min_p), {}};
+    u64 sum = 0;
+    row.each([&](u32 i, float l) { sum += keep(i, l); });
+    sum = block_sum(sh, sum);
+    if (t == 0) {
+      shelf->sums(p.slices)[slice] = sum;
+    }
+    return;
+  }
+  row.each([&](u32, float l) {
+    if (l > -INFINITY) {
+      const int b = x.bin(l);
+      atomicAdd(&sh.count[b], 1u);
+      if (!s.top_k) {
+        atomicAdd(&sh.mass[b], x.weight(l));
+      }
+    }
+  });
+  __syncthreads();
+  if (!s.top_k) {
+    shelf->bins(p.slices, slice)[t] = sh.mass[t];
+    if (sh.mass[t]) {
+      __hip_atomic_fetch_add(&shelf->mass[t], sh.mass[t], __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
+  if (sh.count[t]) {
+    __hip_atomic_fetch_add(&shelf->count[t], sh.count[t], __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+  }
+}
+
+/* The result of a row whose border top_p makes in a bin that is in the list,
+ * with more tokens above it than a list holds: the border, then the slice that
+ * the draw falls in, by the slices' bins, then the token. */
+template <typename R>
+__device__ __forceinline__ void finish_slices(const SampleArgs &a, Shared &sh, int r, R row, const Settings &s,
+                              const Scale &x, const Where &at, const u64 *list, int n,
+                              const Split &p, Shelf *shelf) {
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  auto both = [&](auto take) {
+    for (int j = t; j < n; j += kThreads) {
+      const u32 key = (u32)(list[j] >> 32);
+      take(key, ~(u32)list[j], [&] { return x.weight(logit_of(key)); });
+    }
+  };
+  auto by_key = [&](auto take) { both([&](u32 key, u32, auto weight) { take(key, weight); }); };
+  const u64 want = part_of<true>(s.top_p, at.sum);
+  const Point point = descend<true>(sh, by_key, max(key_of(x.least(at.f.bin)), 1u),
+                                    key_of(x.ftop), at.f.above_mass, 0, want);
+  const Keep<true> keep{x, 0.0, border_at(sh, both, point, ties_of(point.f, want), a.vocab)};
+  /* the kept weight of each slice */
+  __syncthreads();
+  sh.mass[t] = 0;
+  __syncthreads();
+  both([&](u32 key, u32 i, auto weight) {
+    if (keep.border.keeps(key, i)) {
+      atomicAdd(&sh.mass[i / (u32)p.slice], weight());
+    }
+  });
+  for (int sl = wave; sl < p.slices; sl += kWaves) {
+    const u64 *bins = shelf->bins(p.slices, sl);
+    u64 sum = 0;
+    for (int b = lane; b < at.f.bin; b += 64) {
+      sum += bins[b];
+    }
+    sum = wave_sum64(sum);
+    if (lane == 0) {
+      atomicAdd(&sh.mass[sl], sum);
+    }
+  }
+  __syncthreads();
+  const Drawn d = draw_part(sh, sh.mass[t], s.u);
+  row.begin = d.at * p.slice;
+  row.end = min(row.begin + p.slice, a.vocab);
+  draw(a, sh, r, row, s.u, keep, d.total, d.target);
+}
+
+/* The rest: without a border the first slice finds the slice that the draw falls
+ * in and its token; with one, the slices' tokens down to its bin (or, too many, of that bin) meet
+ * in the workspace, and the last slice goes on with them. */
+template <bool kF32> __global__ __launch_bounds__(kThreads) void sample_settle(SampleArgs a, Split p) {
+  __shared__ Shared sh;
+  __shared__ u64 list[kBinList];
+  __shared__ u32 base, last;
+  const int t = threadIdx.x, r = blockIdx.x % a.rows, slice = blockIdx.x / a.rows;
+  Shelf *shelf = reinterpret_cast<Shelf *>(p.ws + r * p.shelf);
+  const Settings s = settings_of(a, r);
+  if (slice != 0 && (s.first || (!s.top_k && s.top_p >= 1.0f))) {
+    return; /* one workgroup is enough */
+  }
+  const u64 first = first_of(sh, shelf, p.slices);
+  const float top = first ? logit_of((u32)(first >> 32)) : -INFINITY;
+  if (!first || s.first) {
+    if (slice == 0) {
+      first_only(a, r, s, top, ~(u32)first);
+    }
+    return;
+  }
+  const Scale x = scale_of(a, s, top);
+  Row<kF32, 0> row(a, r, nullptr);
+  row.inf = x.inf;
+  Row<kF32, 0> mine = row;
+  mine.begin = slice * p.slice;
+  mine.end = min(mine.begin + p.slice, a.vocab);
+  __syncthreads();
+  if (!s.top_k && s.top_p >= 1.0f) {
+    const Drawn d = draw_part(sh, t < p.slices ? shelf->sums(p.slices)[t] : 0, s.u);
+    mine.begin = d.at * p.slice;
+    mine.end = min(mine.begin + p.slice, a.vocab);
+    draw(a, sh, r, mine, s.u, Keep<false>{x, x.share(s.min_p), {}}, d.total,
+         d.target);
+    return;
+  }
+  const Where at = locate(sh, s, shelf->mass[t], shelf->count[t]);
+  const bool few = at.f.bin >= 0 && at.n <= (u32)kList;
+  const bool one_bin = !few && !s.top_k && s.min_p == 0.0f && at.f.count <= (u32)kBinList;
+  if (!few && !one_bin) {
+    if (slice == 0) {
+      finish_bins(a, sh, r, row, s, x, shelf->mass[t], shelf->count[t]);
+    }
+    return;
+  }
+  int n = few ? gather(sh, mine, x, at.bin, list) : gather<true>(sh, mine, x, at.f.bin, list);
+  if (t == 0) {
+    base = __hip_atomic_fetch_add(&shelf->n, (u32)n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  for (int j = t; j < n; j += kThreads) {
+    store_far(&shelf->list[base + j], list[j]);
+  }
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  if (t == 0) {
+    last = __hip_atomic_fetch_add(&shelf->ticket, 1u, __ATOMIC_RELAXED,
+                                  __HIP_MEMORY_SCOPE_AGENT) == (u32)p.slices - 1;
+  }
+  __syncthreads();
+  if (!last) {
+    return;
+  }
+  n = few ? (int)at.n : (int)at.f.count; /* what the slices found in all */
+  for (int j = t; j < n; j += kThreads) {
+    (few ? sh.list_k : list)[j] = load_far(&shelf->list[j]);
+  }
+  __syncthreads();
+  if (few) {
+    finish(a, sh, r, s, x, n, at.sum, at.bin);
+  } else {
+    finish_slices(a, sh, r, row, s, x, at, list, n, p, shelf);
+  }
+}
+
+template <bool kF32> void launch(const SampleArgs &a, const SamplePlan &plan, char *ws, hipStream_t stream) {
   const dim3 grid((unsigned)a.rows), block(kThreads);
+  if (plan.slices > 1) {
+    const Split p{plan.slices, plan.slice, ws, plan.ws_bytes / a.rows};
+    const dim3 all((unsigned)(a.rows * plan.slices));
+    hipLaunchKernelGGL((sample_tops<kF32>), all, block, 0, stream, a, p);
+    hipLaunchKernelGGL((sample_weigh<kF32>), all, block, 0, stream, a, p);
+    hipLaunchKernelGGL((sample_settle<kF32>), all, block, 0, stream, a, p);
+    return;
+  }
   /* the row in LDS where it fits, in two sizes: the smaller leaves room for a
    * second workgroup on a CU */
   constexpr int kSize = kF32 ? 4 : 2;
@@ -855,11 +1262,34 @@ template <bool kF32> void launch(const SampleArgs &a, hipStream_t stream) {
 
 } // namespace
 
-void sample_launch(const SampleArgs &a, hipStream_t stream) {
+/* In us, several workgroups a row and one: 1 x 131072 f32 by top-k 22 and 25, by
+ * top-p 23 and 69, without a border 20 and 48; 100 x 131072 without one 55 and
+ * 59, 150 66 and 60, 256 92 and 73; 256 with one 190 and 226. At 50000 top-k 22
+ * and 16, top-p 23 and 33. Up to 32768 one workgroup has the row in LDS (1 x
+ * 32000 12 and 23). */
+SamplePlan sample_plan(int64_t rows, int64_t vocab, bool borders, bool may_split) {
+  SamplePlan p{1, 0, 0};
+  const int64_t chunks = (vocab + kChunk - 1) / kChunk;
+  if (!may_split || vocab <= 32768 || rows > (borders ? 4096 : 128)) {
+    return p;
+  }
+  /* slices of 1 to 8 chunks, as many as two workgroups a CU of 256 */
+  const int64_t per = std::max<int64_t>(1, std::min<int64_t>(8, rows * chunks / 512));
+  const int64_t slices = (chunks + per - 1) / per;
+  if (slices > kThreads) {
+    return p;
+  }
+  p.slices = (int)slices;
+  p.slice = (int)(per * kChunk);
+  p.ws_bytes = rows * (int64_t)(sizeof(Shelf) + slices * (16 + kBins * 8));
+  return p;
+}
+
+void sample_launch(const SampleArgs &a, const SamplePlan &plan, char *ws, hipStream_t stream) {
   if (a.f32) {
-    launch<true>(a, stream);
+    launch<true>(a, plan, ws, stream);
   } else {
-    launch<false>(a, stream);
+    launch<false>(a, plan, ws, stream);
   }
   VX_HIP_CHECK(hipGetLastError());
 }

@@ -201,8 +201,11 @@ int32_t sample(const char *op, bool f32, const void *logits, const float *temper
   if (on.code != VX_OP_OK) {
     return on.code;
   }
+  const bool borders = top_k || top_p;
+  const Space space(workspace, vxk::sample_plan(rows, vocab, borders, true).ws_bytes);
   vxk::sample_launch(vxk::SampleArgs{logits, temperature, top_k, top_p, min_p, u, tokens, logprob,
                                      (int)rows, (int)vocab, stride, f32},
+                     vxk::sample_plan(rows, vocab, borders, space.enough), space.base,
                      vxops::stream());
   vxops::launched(op);
   return VX_OP_OK;
@@ -322,7 +325,7 @@ int64_t vx_nn_sample_workspace(int64_t rows, int64_t vocab) {
   if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > (int64_t(1) << 30)) {
     return VX_OP_EINVAL;
   }
-  return 0;
+  return vxk::sample_plan(rows, vocab, true, true).ws_bytes;
 }
 
 int32_t vx_nn_sample_f32(const float *logits, const float *temperature, const int32_t *top_k,

@@ -67,7 +67,16 @@ struct SampleArgs {
   int64_t stride;
   bool f32;
 };
-void sample_launch(const SampleArgs &a, hipStream_t stream);
+/* `slices` workgroups a row of `slice` logits each (1: one a row, which needs no
+ * workspace). */
+struct SamplePlan {
+  int slices, slice;
+  int64_t ws_bytes;
+};
+/* Plain host arithmetic; `borders`: top_k or top_p may be on in a row;
+ * `may_split` false: a plan without a workspace. */
+SamplePlan sample_plan(int64_t rows, int64_t vocab, bool borders, bool may_split);
+void sample_launch(const SampleArgs &a, const SamplePlan &plan, char *ws, hipStream_t stream);
 
 } // namespace vxk
 
