@@ -261,6 +261,22 @@ int32_t vx_llama_i8_generate(void *model, const int32_t *prompt,
                              int32_t *out_tokens, float *out_margin,
                              int32_t flags);
 
+/* The same with tokens drawn as vx_nn_sample_f32 draws them, by the given
+ * settings (values that turn a setting off: temperature 1, top_k 0, top_p 1,
+ * min_p 0; temperature 0 is greedy) and u[i] for the i-th generated token.
+ * out_logprob (may be NULL) gets the natural logarithm of each token's share of
+ * the kept weight; where every logit is NaN the token is -1 and generation goes
+ * on from token 0. */
+typedef struct vx_llama_sampling {
+  float temperature;
+  int32_t top_k;
+  float top_p, min_p;
+} vx_llama_sampling;
+int32_t vx_llama_i8_sample(void *model, const int32_t *prompt, int32_t n_prompt,
+                           int32_t n_steps, const vx_llama_sampling *how,
+                           const float *u, int32_t *out_tokens,
+                           float *out_logprob, int32_t flags);
+
 /* Feed tokens[0..n) at positions 0..n-1 and copy the logits after each
  * position to logits[n, vocab]. Returns 0 or a VX_OP_E* code. */
 int32_t vx_llama_i8_logits(void *model, const int32_t *tokens, int32_t n,

@@ -15,6 +15,7 @@
  */
 #include "../../include/vx_hardware_runtime.h"
 #include "../../include/vx_hip_ops.h"
+#include "vx_batch_kernels.h"
 #include "vx_decode_kernels.h"
 #include "vx_hip_common.h"
 #include "vx_kernels.h"
@@ -43,6 +44,16 @@ constexpr int kGraphSteps = VX_DEC_GRAPH_STEPS;
 constexpr int kPrefillMin = 3;
 constexpr int kScoreMin = 2;
 
+/* The instantiated step graphs (one step, kGraphSteps steps; [1]: for steps
+ * whose positions are all below step_attention_near, whose attention takes
+ * smaller rounds of rows), kept across calls: they bake in the prompt length
+ * and the I/O buffers, so they are dropped when either changes. */
+struct StepGraphs {
+  hipGraphExec_t step[2] = {nullptr, nullptr};
+  hipGraphExec_t steps[2] = {nullptr, nullptr};
+  int prompt = -1;
+};
+
 struct LlamaI8 {
   vx_llama_i8_config cfg;
   int hs = 0, kv_dim = 0, device = 0;
@@ -69,14 +80,15 @@ struct LlamaI8 {
   char *staging = nullptr;
   hipEvent_t arrived[2] = {nullptr, nullptr};
   hipStream_t stream = nullptr;
-  /* The instantiated step graphs (one step, kGraphSteps steps; [1]: for
-   * steps whose positions are all below step_attention_near, whose
-   * attention takes smaller rounds of rows), kept across generate calls:
-   * they bake in the prompt length and the I/O buffers, so they are dropped
-   * when either changes. */
-  hipGraphExec_t step_exec[2] = {nullptr, nullptr};
-  hipGraphExec_t steps_exec[2] = {nullptr, nullptr};
-  int step_exec_prompt = -1;
+  StepGraphs graphs[2]; /* greedy, sampled */
+  /* Sampled generation (taken when first asked for): the settings, the uniform
+   * numbers, the drawn token as the one candidate (its log-probability as the
+   * lead over a runner-up at 0), and the workspace of a large vocabulary. */
+  vx_llama_sampling *how = nullptr;
+  float *uniform = nullptr;
+  vxk::StepBest *drawn = nullptr;
+  char *sample_ws = nullptr;
+  int uniform_cap = 0;
   std::vector<void *> owned;
 };
 
@@ -94,15 +106,21 @@ template <typename T> T *alloc(LlamaI8 &m, size_t count) {
   return upload<T>(m, nullptr, count);
 }
 
-void drop_step_graph(LlamaI8 &m) {
-  for (hipGraphExec_t *g : {&m.step_exec[0], &m.step_exec[1], &m.steps_exec[0],
-                            &m.steps_exec[1]}) {
+void drop_step_graphs(StepGraphs &graphs) {
+  for (hipGraphExec_t *g : {&graphs.step[0], &graphs.step[1], &graphs.steps[0],
+                            &graphs.steps[1]}) {
     if (*g) {
       (void)hipGraphExecDestroy(*g);
       *g = nullptr;
     }
   }
-  m.step_exec_prompt = -1;
+  graphs.prompt = -1;
+}
+
+void drop_step_graph(LlamaI8 &m) {
+  for (StepGraphs &g : m.graphs) {
+    drop_step_graphs(g);
+  }
 }
 
 void release(LlamaI8 &m) {
@@ -145,10 +163,10 @@ bool ensure_io(LlamaI8 &m, int n_prompt, int n_out) {
   return true;
 }
 
-vxk::StepTokenArgs token_args(LlamaI8 &m, int n_prompt) {
+vxk::StepTokenArgs token_args(LlamaI8 &m, int n_prompt, bool sampled) {
   vxk::StepTokenArgs a;
-  a.cand = m.best;
-  a.ncand = vxk::step_logits_groups(m.cfg.vocab_size);
+  a.cand = sampled ? m.drawn : m.best;
+  a.ncand = sampled ? 1 : vxk::step_logits_groups(m.cfg.vocab_size);
   a.prompt = m.prompt;
   a.n_prompt = n_prompt;
   a.out_tokens = m.out_tokens;
@@ -160,9 +178,9 @@ vxk::StepTokenArgs token_args(LlamaI8 &m, int n_prompt) {
   return a;
 }
 
-vxk::StepArgmaxArgs argmax_args(LlamaI8 &m, int n_prompt) {
+vxk::StepArgmaxArgs argmax_args(LlamaI8 &m, int n_prompt, bool sampled) {
   vxk::StepArgmaxArgs a;
-  a.tok = token_args(m, n_prompt);
+  a.tok = token_args(m, n_prompt, sampled);
   a.pos = m.pos;
   return a;
 }
@@ -183,9 +201,21 @@ void enqueue_classifier(LlamaI8 &m, const float *x) {
   vxk::step_gemv_logits(lg, m.stream);
 }
 
+/* The token after the position whose logits the classifier left, drawn by the
+ * model's settings and the position's uniform number. */
+void enqueue_draw(LlamaI8 &m, int n_prompt) {
+  vxk::SampleArgs a{m.logits, &m.how->temperature, &m.how->top_k, &m.how->top_p, &m.how->min_p,
+                    m.uniform, &m.drawn->i1, &m.drawn->v1, 1, m.cfg.vocab_size,
+                    m.cfg.vocab_size, true};
+  a.step = m.pos;
+  a.step0 = n_prompt;
+  vxk::sample_launch(a, vxk::sample_plan(1, m.cfg.vocab_size, true, m.sample_ws != nullptr),
+                     m.sample_ws, m.stream);
+}
+
 /* One token step on the model's stream; `near`: its position is below
  * step_attention_near (the attention launches take smaller rounds). */
-void enqueue_step(LlamaI8 &m, int n_prompt, bool near) {
+void enqueue_step(LlamaI8 &m, int n_prompt, bool near, bool sampled) {
   const vx_llama_i8_config &c = m.cfg;
   const int qkv_rows = c.dim + 2 * m.kv_dim;
   const int64_t layer_kv = (int64_t)c.seq_len * m.kv_dim;
@@ -210,7 +240,7 @@ void enqueue_step(LlamaI8 &m, int n_prompt, bool near) {
     if (l == 0) {
       /* the position's token and its embedding as x; the rotary row */
       vxk::StepEmbedArgs e;
-      e.tok = token_args(m, n_prompt);
+      e.tok = token_args(m, n_prompt, sampled);
       e.xout = m.x;
       e.rope_table = m.rope;
       e.rope_out = m.rope_now;
@@ -261,6 +291,9 @@ void enqueue_step(LlamaI8 &m, int n_prompt, bool near) {
     vxk::step_gemv_resid(w2, m.stream);
   }
   enqueue_classifier(m, m.x);
+  if (sampled) {
+    enqueue_draw(m, n_prompt);
+  }
 }
 
 /* Positions pos0 .. pos0 + count - 1 (count at most kPrefillCap) of the
@@ -369,6 +402,120 @@ void read_back(LlamaI8 &m, char *dst, const char *src, size_t bytes) {
       memcpy(dst + (i - 1) * kStagingPiece, m.staging + (i - 1) % 2 * kStagingPiece, size(i - 1));
     }
   }
+}
+
+/* The settings and `n` uniform numbers to the GPU. */
+void upload_sampling(LlamaI8 &m, const vx_llama_sampling *how, const float *u, int n) {
+  if (!m.how) {
+    m.how = alloc<vx_llama_sampling>(m, 1);
+    const vxk::StepBest none{0.0f, 0, 0.0f};
+    m.drawn = upload<vxk::StepBest>(m, &none, 1);
+    /* the null stream's copy, before the model's own takes it up */
+    VX_HIP_CHECK(hipStreamSynchronize(nullptr));
+    const int64_t bytes = vxk::sample_plan(1, m.cfg.vocab_size, true, true).ws_bytes;
+    if (bytes) {
+      m.sample_ws = alloc<char>(m, (size_t)bytes);
+    }
+  }
+  if (n > m.uniform_cap) {
+    m.uniform = alloc<float>(m, (size_t)n);
+    m.uniform_cap = n;
+    drop_step_graphs(m.graphs[1]);
+  }
+  VX_HIP_CHECK(hipMemcpyAsync(m.how, how, sizeof *how, hipMemcpyHostToDevice, m.stream));
+  VX_HIP_CHECK(hipMemcpyAsync(m.uniform, u, sizeof(float) * (size_t)n, hipMemcpyHostToDevice,
+                              m.stream));
+}
+
+/* vx_llama_i8_generate, and with settings vx_llama_i8_sample. */
+int32_t generate(LlamaI8 *m, const int32_t *prompt, int32_t n_prompt, int32_t n_steps,
+                 const vx_llama_sampling *how, const float *u, int32_t *out_tokens,
+                 float *out_margin, int32_t flags) {
+  const bool sampled = how != nullptr;
+  if (!m || !prompt || !out_tokens || n_prompt < 1 || n_steps < 1) {
+    return refuse(VX_OP_EINVAL, "need a model, a prompt of at least one "
+                                "token and at least one step");
+  }
+  if (n_prompt + n_steps - 1 > m->cfg.seq_len) {
+    return refuse(VX_OP_EINVAL, "prompt + steps exceed the model's seq_len");
+  }
+  for (int i = 0; i < n_prompt; ++i) {
+    if (prompt[i] < 0 || prompt[i] >= m->cfg.vocab_size) {
+      return refuse(VX_OP_EINVAL, "a prompt token is outside the vocabulary");
+    }
+  }
+  VX_HIP_CHECK(hipSetDevice(m->device));
+  ensure_io(*m, n_prompt, n_steps);
+  VX_HIP_CHECK(hipMemcpyAsync(m->prompt, prompt, sizeof(int) * n_prompt,
+                              hipMemcpyHostToDevice, m->stream));
+  if (sampled) {
+    upload_sampling(*m, how, u, n_steps);
+  }
+  vxk::StepArgmaxArgs start = argmax_args(*m, n_prompt, sampled);
+  const int positions = n_prompt + n_steps - 1;
+  const int near_pos = vxk::step_attention_near(m->hs);
+  int p = 0; /* the first position that takes a step of its own */
+  if (n_prompt >= kPrefillMin) {
+    int count = 0;
+    for (; p < n_prompt; p += count) {
+      count = std::min(n_prompt - p, vxk::kPrefillCap);
+      enqueue_prefill(*m, p, count);
+    }
+    vxk::fill_i32_launch(m->pos, n_prompt - 1, m->stream);
+    enqueue_classifier(*m, m->px + (int64_t)(count - 1) * m->cfg.dim);
+    if (sampled) {
+      enqueue_draw(*m, n_prompt);
+    }
+  } else {
+    vxk::step_start_launch(start, m->stream);
+  }
+  if (flags & VX_LLAMA_GRAPH) {
+    StepGraphs &graphs = m->graphs[sampled];
+    if (graphs.prompt != n_prompt) {
+      drop_step_graphs(graphs);
+      graphs.prompt = n_prompt;
+    }
+    /* the graph of `steps` steps for positions p .. p + steps - 1,
+     * captured when first needed */
+    auto graph_for = [&](int p, int steps) {
+      const int near = p + steps - 1 < near_pos ? 1 : 0;
+      hipGraphExec_t &exec = steps == 1 ? graphs.step[near] : graphs.steps[near];
+      if (!exec) {
+        hipGraph_t graph = nullptr;
+        VX_HIP_CHECK(hipStreamBeginCapture(m->stream, hipStreamCaptureModeThreadLocal));
+        for (int i = 0; i < steps; ++i) {
+          enqueue_step(*m, n_prompt, near != 0, sampled);
+        }
+        VX_HIP_CHECK(hipStreamEndCapture(m->stream, &graph));
+        VX_HIP_CHECK(hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0));
+        VX_HIP_CHECK(hipGraphDestroy(graph));
+      }
+      return exec;
+    };
+    for (; kGraphSteps > 1 && p + kGraphSteps <= positions; p += kGraphSteps) {
+      VX_HIP_CHECK(hipGraphLaunch(graph_for(p, kGraphSteps), m->stream));
+    }
+    for (; p < positions; ++p) {
+      VX_HIP_CHECK(hipGraphLaunch(graph_for(p, 1), m->stream));
+    }
+  } else {
+    for (; p < positions; ++p) {
+      enqueue_step(*m, n_prompt, p < near_pos, sampled);
+    }
+  }
+  /* the token after the last step */
+  vxk::step_record_launch(start, m->stream);
+  VX_HIP_CHECK(hipGetLastError());
+  VX_HIP_CHECK(hipMemcpyAsync(out_tokens, m->out_tokens,
+                              sizeof(int) * n_steps, hipMemcpyDeviceToHost,
+                              m->stream));
+  if (out_margin) {
+    VX_HIP_CHECK(hipMemcpyAsync(out_margin, m->out_margin,
+                                sizeof(float) * n_steps,
+                                hipMemcpyDeviceToHost, m->stream));
+  }
+  VX_HIP_CHECK(hipStreamSynchronize(m->stream));
+  return VX_OP_OK;
 }
 
 } // namespace
@@ -497,84 +644,18 @@ int32_t vx_llama_i8_generate(void *model, const int32_t *prompt,
                              int32_t n_prompt, int32_t n_steps,
                              int32_t *out_tokens, float *out_margin,
                              int32_t flags) {
-  LlamaI8 *m = static_cast<LlamaI8 *>(model);
-  if (!m || !prompt || !out_tokens || n_prompt < 1 || n_steps < 1) {
-    return refuse(VX_OP_EINVAL, "need a model, a prompt of at least one "
-                                "token and at least one step");
+  return generate(static_cast<LlamaI8 *>(model), prompt, n_prompt, n_steps, nullptr, nullptr,
+                  out_tokens, out_margin, flags);
+}
+
+int32_t vx_llama_i8_sample(void *model, const int32_t *prompt, int32_t n_prompt,
+                           int32_t n_steps, const vx_llama_sampling *how, const float *u,
+                           int32_t *out_tokens, float *out_logprob, int32_t flags) {
+  if (!how || !u) {
+    return refuse(VX_OP_EINVAL, "need the sampling settings and a uniform number per step");
   }
-  if (n_prompt + n_steps - 1 > m->cfg.seq_len) {
-    return refuse(VX_OP_EINVAL, "prompt + steps exceed the model's seq_len");
-  }
-  for (int i = 0; i < n_prompt; ++i) {
-    if (prompt[i] < 0 || prompt[i] >= m->cfg.vocab_size) {
-      return refuse(VX_OP_EINVAL, "a prompt token is outside the vocabulary");
-    }
-  }
-  VX_HIP_CHECK(hipSetDevice(m->device));
-  ensure_io(*m, n_prompt, n_steps);
-  VX_HIP_CHECK(hipMemcpyAsync(m->prompt, prompt, sizeof(int) * n_prompt,
-                              hipMemcpyHostToDevice, m->stream));
-  vxk::StepArgmaxArgs start = argmax_args(*m, n_prompt);
-  const int positions = n_prompt + n_steps - 1;
-  const int near_pos = vxk::step_attention_near(m->hs);
-  int p = 0; /* the first position that takes a step of its own */
-  if (n_prompt >= kPrefillMin) {
-    int count = 0;
-    for (; p < n_prompt; p += count) {
-      count = std::min(n_prompt - p, vxk::kPrefillCap);
-      enqueue_prefill(*m, p, count);
-    }
-    vxk::fill_i32_launch(m->pos, n_prompt - 1, m->stream);
-    enqueue_classifier(*m, m->px + (int64_t)(count - 1) * m->cfg.dim);
-  } else {
-    vxk::step_start_launch(start, m->stream);
-  }
-  if (flags & VX_LLAMA_GRAPH) {
-    if (m->step_exec_prompt != n_prompt) {
-      drop_step_graph(*m);
-      m->step_exec_prompt = n_prompt;
-    }
-    /* the graph of `steps` steps for positions p .. p + steps - 1,
-     * captured when first needed */
-    auto graph_for = [&](int p, int steps) {
-      const int near = p + steps - 1 < near_pos ? 1 : 0;
-      hipGraphExec_t &exec = steps == 1 ? m->step_exec[near] : m->steps_exec[near];
-      if (!exec) {
-        hipGraph_t graph = nullptr;
-        VX_HIP_CHECK(hipStreamBeginCapture(m->stream, hipStreamCaptureModeThreadLocal));
-        for (int i = 0; i < steps; ++i) {
-          enqueue_step(*m, n_prompt, near != 0);
-        }
-        VX_HIP_CHECK(hipStreamEndCapture(m->stream, &graph));
-        VX_HIP_CHECK(hipGraphInstantiate(&exec, graph, nullptr, nullptr, 0));
-        VX_HIP_CHECK(hipGraphDestroy(graph));
-      }
-      return exec;
-    };
-    for (; kGraphSteps > 1 && p + kGraphSteps <= positions; p += kGraphSteps) {
-      VX_HIP_CHECK(hipGraphLaunch(graph_for(p, kGraphSteps), m->stream));
-    }
-    for (; p < positions; ++p) {
-      VX_HIP_CHECK(hipGraphLaunch(graph_for(p, 1), m->stream));
-    }
-  } else {
-    for (; p < positions; ++p) {
-      enqueue_step(*m, n_prompt, p < near_pos);
-    }
-  }
-  /* the token after the last step */
-  vxk::step_record_launch(start, m->stream);
-  VX_HIP_CHECK(hipGetLastError());
-  VX_HIP_CHECK(hipMemcpyAsync(out_tokens, m->out_tokens,
-                              sizeof(int) * n_steps, hipMemcpyDeviceToHost,
-                              m->stream));
-  if (out_margin) {
-    VX_HIP_CHECK(hipMemcpyAsync(out_margin, m->out_margin,
-                                sizeof(float) * n_steps,
-                                hipMemcpyDeviceToHost, m->stream));
-  }
-  VX_HIP_CHECK(hipStreamSynchronize(m->stream));
-  return VX_OP_OK;
+  return generate(static_cast<LlamaI8 *>(model), prompt, n_prompt, n_steps, how, u, out_tokens,
+                  out_logprob, flags);
 }
 
 int32_t vx_llama_i8_logits(void *model, const int32_t *tokens, int32_t n,
@@ -619,10 +700,10 @@ int32_t vx_llama_i8_logits(void *model, const int32_t *tokens, int32_t n,
     }
     return VX_OP_OK;
   }
-  vxk::step_start_launch(argmax_args(*m, n), m->stream);
+  vxk::step_start_launch(argmax_args(*m, n, false), m->stream);
   const int near_pos = vxk::step_attention_near(m->hs);
   for (int p = 0; p < n; ++p) {
-    enqueue_step(*m, n, p < near_pos);
+    enqueue_step(*m, n, p < near_pos, false);
     VX_HIP_CHECK(hipMemcpyAsync(logits + p * vocab, m->logits,
                                 sizeof(float) * vocab, hipMemcpyDeviceToHost,
                                 m->stream));

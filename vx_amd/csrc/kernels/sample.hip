@@ -88,7 +88,7 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs &a, int r) {
   const int top_k = a.top_k ? a.top_k[r] : 0;
   const float top_p = a.top_p ? a.top_p[r] : 1.0f;
   const float min_p = a.min_p ? a.min_p[r] : 0.0f;
-  const float u = a.u[r];
+  const float u = a.u[a.step ? max(*a.step - a.step0, 0) : r];
   Settings s;
   s.u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
   s.first = !(heat > 0.0f) || top_k == 1 || top_p <= 0.0f;

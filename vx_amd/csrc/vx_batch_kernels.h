@@ -66,6 +66,10 @@ struct SampleArgs {
   int rows, vocab;
   int64_t stride;
   bool f32;
+  /* Where not NULL, the one row's uniform number is u[*step - step0] (u[0]
+   * before step0). */
+  const int *step = nullptr;
+  int step0 = 0;
 };
 /* `slices` workgroups a row of `slice` logits each (1: one a row, which needs no
  * workspace). */

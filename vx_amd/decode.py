@@ -1,7 +1,8 @@
-"""Greedy int8 decode on the GPU through vx_llama_i8_* (include/vx_hip_ops.h).
+"""Int8 decode on the GPU, greedy or sampled, through vx_llama_i8_* (include/vx_hip_ops.h).
 
     model = LlamaI8(lib, cfg, weights)     # upload (weights from vx_amd.llama)
     tokens, margin = model.generate(prompt, n_steps)
+    tokens, logprob = model.sample(prompt, u, temperature=0.8, top_p=0.95)
     logits = model.logits(tokens)          # per position, for parity checks
     cfg, weights = read_model(lib, path)   # a llama2.c checkpoint or VXQ8 file
 """
@@ -24,6 +25,11 @@ GRAPH = 1
 class _Config(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in
                 ("dim", "hidden_dim", "n_layers", "n_heads", "n_kv_heads", "vocab_size", "seq_len")]
+
+
+class _Sampling(ctypes.Structure):
+    _fields_ = [("temperature", ctypes.c_float), ("top_k", ctypes.c_int32), ("top_p", ctypes.c_float),
+                ("min_p", ctypes.c_float)]
 
 
 class _Weights(ctypes.Structure):
@@ -126,6 +132,22 @@ class LlamaI8:
             raise RuntimeError(f"vx_llama_i8_generate returned {rc}")
         return toks, margin
 
+    def sample(self, prompt, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+               min_p: float = 0.0, graph: bool = True):
+        """As many tokens as `u` has uniform numbers, drawn by vx_nn_sample_f32's
+        rules, and the logarithm of each one's share of the kept weight."""
+        prompt = np.ascontiguousarray(prompt, np.int32)
+        u = np.ascontiguousarray(u, np.float32)
+        toks = np.empty(len(u), np.int32)
+        logprob = np.empty(len(u), np.float32)
+        how = _Sampling(temperature, top_k, top_p, min_p)
+        rc = self.lib.lib.vx_llama_i8_sample(self.handle, prompt.ctypes.data, len(prompt), len(u),
+                                             ctypes.byref(how), u.ctypes.data, toks.ctypes.data,
+                                             logprob.ctypes.data, GRAPH if graph else 0)
+        if rc != 0:
+            raise RuntimeError(f"vx_llama_i8_sample returned {rc}")
+        return toks, logprob
+
     def logits(self, tokens) -> np.ndarray:
         tokens = np.ascontiguousarray(tokens, np.int32)
         out = np.empty((len(tokens), self.cfg.vocab_size), np.float32)
@@ -190,6 +212,7 @@ def main(argv=None) -> int:
     program a kernel trace of the decode step profiles.
 
         python -m vx_amd.decode [--steps N] [--eager] [--lib PATH]
+            [--temperature T [--top-k K] [--top-p P] [--min-p M] [--seed S]]
     """
     import argparse
 
@@ -200,15 +223,27 @@ def main(argv=None) -> int:
     ap.add_argument("--eager", action="store_true",
                     help="launch the step's kernels one by one instead of replaying a hipGraph")
     ap.add_argument("--lib", default=str(LIB_PATH))
+    ap.add_argument("--temperature", type=float, default=0.0, help="sample; 0 (the default): greedy")
+    ap.add_argument("--top-k", type=int, default=0)
+    ap.add_argument("--top-p", type=float, default=1.0)
+    ap.add_argument("--min-p", type=float, default=0.0)
+    ap.add_argument("--seed", type=int, default=0, help="of the uniform numbers that tokens are drawn with")
     ns = ap.parse_args(argv)
     lib = DispatchLibrary(ns.lib)
     cfg = CONFIG_DECODE
     model = LlamaI8(lib, cfg, make_model(cfg, seed=0))
     try:
         prompt = make_prompt(cfg, n=16, seed=1)
-        model.generate(prompt, 4, graph=not ns.eager)  # warm
+        def tokens(n):
+            if ns.temperature <= 0:
+                return model.generate(prompt, n, graph=not ns.eager)[0]
+            u = np.random.default_rng(ns.seed).random(n, dtype=np.float32)
+            return model.sample(prompt, u, ns.temperature, ns.top_k, ns.top_p, ns.min_p,
+                                graph=not ns.eager)[0]
+
+        tokens(4)  # warm
         t0 = time.perf_counter()
-        toks, _ = model.generate(prompt, ns.steps, graph=not ns.eager)
+        toks = tokens(ns.steps)
         dt = time.perf_counter() - t0
     finally:
         model.close()

@@ -74,6 +74,7 @@ HIP_SIGNATURES = {
     "vx_nn_sample_workspace": (_i64, [_i64, _i64]),
     "vx_llama_i8_create": (_vp, [_vp, _vp, _u32]),
     "vx_llama_i8_generate": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _i32]),
+    "vx_llama_i8_sample": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32]),
     "vx_llama_i8_logits": (_i32, [_vp, _vp, _i32, _vp]),
     "vx_llama_i8_destroy": (None, [_vp]),
     "vx_llama_i8_read": (_i32, [ctypes.c_char_p, _vp, ctypes.POINTER(_vp)]),
