@@ -88,8 +88,9 @@ int32_t vx_nn_gemv_i8_bf16(const int8_t *w, const float *scale,
  * sequence has, the step's seq_q new ones among them: query i of sequence b is
  * at position shared_len + lens[b] - seq_q + i. It is read when the kernels
  * run, so a captured graph follows it. lens NULL: capacity for all. A slot
- * whose lens[b] is negative or above capacity holds no sequence: nothing of it
- * is read, and its outputs and cache stay as they were.
+ * whose lens[b] is negative or above capacity holds no sequence: what it has
+ * for queries and cache does not matter, and its outputs and cache stay as they
+ * were.
  *
  * Arguments are checked before the GPU is looked for, so a refusal is the same
  * without one. Every pointer must be memory of one GPU; the ops run on that
@@ -99,9 +100,12 @@ int32_t vx_nn_gemv_i8_bf16(const int8_t *w, const float *scale,
  * of no account before and after. The calls work with NULL: then the library
  * keeps a block per (device, stream), taken and freed as attention's split
  * workspaces are, and a stream that is capturing a graph, or hipStreamPerThread,
- * gets a launch that needs none. A captured call that shall divide its work
- * is given one of at least *_workspace() bytes (a smaller one is refused),
- * which two launches that may run at the same time must not share. */
+ * gets a launch that needs none (slower: each sequence reads the shared keys
+ * itself, one workgroup draws each row). A captured call that shall divide its
+ * work is given one of at least *_workspace() bytes (a smaller one is refused),
+ * which two launches that may run at the same time must not share. Sampling
+ * uses at most 1024 x (45 KiB + 8.2 KiB per 32768 logits), attention 4 *
+ * (head_dim + 2) bytes a query of a head for each part of the keys. */
 
 /* Splits, rotates and appends. qkv: [batch, seq_q, heads + 2 * kv_heads,
  * head_dim] (a token's queries, keys and values together, as one projection
@@ -184,7 +188,7 @@ int64_t vx_nn_flash_attention_shared_workspace(int64_t batch, int64_t heads,
  * Weights are 64-bit integers in units of at most 2^-32 of the row's largest
  * one (2^-45 at a vocabulary of 131072), so sums are exact and a result does
  * not depend on how the work is divided; a token whose weight rounds to 0 is
- * not drawn. vocab at most 2^30. */
+ * not drawn. rows at most 2^21, vocab at most 2^30. */
 int32_t vx_nn_sample_f32(const float *logits, const float *temperature,
                          const int32_t *top_k, const float *top_p,
                          const float *min_p, const float *u, int32_t *tokens,

@@ -127,15 +127,20 @@ def run(a, steps, step, check=False):
         a.put("x", a.emb[out[-1]])
         a.put("lens", lens)
         a.put("u", a.u[s])
-        before = [bf16_to_f32(dev[x].numpy()).astype(np.float64) for x in ("q", "k", "v")] if check else None
+        before = [dev[x].numpy().copy() for x in ("q", "k", "v")] if check else None
         o_before = dev["o"].numpy().copy() if check else None
         step()
         tokens = dev["tokens"].numpy().copy()
         if check:
             qkv = bf16_to_f32(dev["qkv"].numpy()).reshape(b, 1, h + 2 * kv, d)
-            want, tol = ref.rope_append(qkv, a.table, lens, *before, n)
-            for name, w, t in zip(("q", "k", "v"), want, tol):
-                assert np.all(np.abs(bf16_to_f32(dev[name].numpy()) - w) <= t), (s, name)
+            # what memory held before, whatever it was, stays as it was
+            held = [np.zeros(x.shape) for x in before]
+            want, tol = ref.rope_append(qkv, a.table, lens, *held, n)
+            touched, _ = ref.rope_append(np.ones_like(qkv), None, lens, *held, n)
+            for name, w, t, b16, new in zip(("q", "k", "v"), want, tol, before, touched):
+                got = dev[name].numpy()
+                assert np.array_equal(got[new == 0], b16[new == 0]), (s, name)
+                assert np.all(np.abs(bf16_to_f32(got) - w)[new == 1] <= t[new == 1]), (s, name)
             (wo, _), (to, _) = ref.shared_attention(dev["q"].numpy(), dev["ks"].numpy(), dev["vs"].numpy(),
                                                     dev["k"].numpy(), dev["v"].numpy(), lens, n, d ** -0.5, True)
             o = dev["o"].numpy()

@@ -295,3 +295,68 @@ def test_two_streams_at_once(hiplib):
             c.free()
         for s in streams:
             t.stream_destroy(s)
+
+
+def test_per_thread_stream(hiplib):
+    """hipStreamPerThread names a stream per thread: calls under it take no
+    workspace of the library's, and two threads' calls run at once."""
+    import threading
+    announce("flash_shared under hipStreamPerThread")
+    t = HipTimer()
+    case = (40, 8, 2, 1, 1200, 40, 64, [i % 41 for i in range(40)])
+    calls = [Call(hiplib, *case, seed=i) for i in range(2)]
+    wants = [c.want() for c in calls]
+    t.sync()
+    failed = []
+
+    def work(c):
+        try:
+            hiplib.lib.vx_hip_set_stream(2)  # hipStreamPerThread
+            for _ in range(5):
+                c()
+            hiplib.lib.vx_hip_set_stream(None)
+        except BaseException as e:  # noqa: BLE001 - reported below
+            failed.append(e)
+
+    before = held(hiplib)
+    threads = [threading.Thread(target=work, args=(c,)) for c in calls]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    t.sync()
+    assert not failed
+    assert held(hiplib) == before
+    for c, w in zip(calls, wants):
+        c.check(w)
+        c.free()
+
+
+def held(lib):
+    """The workspaces that the library keeps, and their bytes."""
+    import ctypes
+    out = (ctypes.c_int64 * 2)()
+    assert lib.control(abi.HIP_CTRL_OP_WORKSPACES, out) == 1
+    return tuple(out)
+
+
+def test_a_streams_workspace_goes_with_it(hiplib):
+    announce("flash_shared workspace of a stream")
+    t = HipTimer()
+    stream = t.stream_create()
+    c = Call(hiplib, 64, 8, 2, 1, 1500, 40, 128, [i % 41 for i in range(64)])
+    before = held(hiplib)
+    try:
+        hiplib.lib.vx_hip_set_stream(stream)
+        c()
+        assert held(hiplib)[0] == before[0] + 1
+        assert held(hiplib)[1] >= before[1] + c.workspace_bytes() > before[1]
+        c(), t.sync()
+        assert held(hiplib)[0] == before[0] + 1
+    finally:
+        hiplib.lib.vx_hip_set_stream(None)
+    assert held(hiplib) == before
+    t.sync()
+    c.check()
+    c.free()
+    t.stream_destroy(stream)

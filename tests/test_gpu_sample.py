@@ -248,3 +248,62 @@ def test_without_logprob_and_back_to_back(hiplib):
             c.check(w)
     for c in calls:
         c.free()
+
+
+def test_many_rows_of_a_large_vocabulary(hiplib):
+    """More rows than workgroups share one of: with and without borders."""
+    announce("sample many rows")
+    rng = np.random.default_rng(12)
+    for rows, vocab in ((130, 40000), (1030, 33000)):
+        x = likely(rng, rows, vocab, top=9.0)
+        u = rng.random(rows, dtype=np.float32)
+        check(hiplib, x, u, dtype="bf16")
+        check(hiplib, x, u, top_p=np.where(np.arange(rows) % 2 == 0, 0.9, 1), top_k=np.where(np.arange(rows) % 3 == 0, 30, 0))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [5000, 70000])
+def test_wide_borders(hiplib, vocab, dtype):
+    """Borders with more tokens above them, in their bin and at their logit than a
+    list holds."""
+    announce(f"sample wide borders {vocab} {dtype}")
+    rng = np.random.default_rng(vocab)
+    rows = 10
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    x[0] = 0
+    x[1] = np.round(x[1])
+    x[2] = x[2] * 1e-3 + 5
+    x[3, ::2] = 1.25
+    x[4] = np.where(rng.random(vocab) < 0.5, 3.0, x[4])
+    x[5] *= 30
+    u = rng.random(rows, dtype=np.float32)
+    for kw in (dict(top_p=0.5), dict(top_p=0.999), dict(top_k=vocab // 2), dict(top_k=vocab - 1, top_p=0.7),
+               dict(top_k=1500, top_p=0.99, min_p=0.5), dict(min_p=0.4), dict(top_p=0.9, min_p=1e-3, temperature=3.0)):
+        check(hiplib, x, u, dtype=dtype, **kw)
+
+
+def test_two_streams_at_once(hiplib):
+    announce("sample on two streams")
+    t = HipTimer()
+    rng = np.random.default_rng(3)
+    streams = [t.stream_create() for _ in range(2)]
+    calls = [Call(hiplib, likely(rng, 20, 50000 + i), rng.random(20, dtype=np.float32), top_p=0.95,
+                  temperature=0.9 + i) for i in range(2)]
+    wants = [c.want() for c in calls]
+    t.sync()
+    try:
+        for _ in range(10):
+            for s, c in zip(streams, calls):
+                hiplib.lib.vx_hip_set_stream(s)
+                c()
+        t.sync()
+        hiplib.lib.vx_hip_set_stream(None)
+        for c, w in zip(calls, wants):
+            c.check(w)
+    finally:
+        hiplib.lib.vx_hip_set_stream(None)
+        t.sync()
+        for c in calls:
+            c.free()
+        for s in streams:
+            t.stream_destroy(s)

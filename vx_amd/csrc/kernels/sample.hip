@@ -102,9 +102,9 @@ __device__ __forceinline__ Settings settings_of(const SampleArgs &a, int r) {
 
 /* How a row's logits become weights. Where a logit is +inf, those count as 0
  * and the others as -inf.
- * 2^d, d <= 0, in units: with k the integer next to d, 2^(d - k) = e^x, |x| <=
- * ln(2) / 2, by its Taylor sum to the 12th power (what is left out is below
- * 2^-52), and 2^k by an addition to the exponent. Adding 1.5 * 2^52 to d leaves k
+ * 2^d, d <= 0, in units: with k the integer next to d, 2^(d - k) by the
+ * polynomial of degree 10 that meets 2^f at the 11 Chebyshev nodes of [-1/2, 1/2]
+ * (off by at most 2^-51.5), and 2^k by an addition to the exponent. Adding 1.5 * 2^52 to d leaves k
  * in the low bits: conversions and roundings of 64 bits take four times an
  * addition's cycles, and a table in LDS twice a longer sum's. */
 struct Scale {
@@ -118,20 +118,16 @@ struct Scale {
     const double d = fmax(((double)l - top) * c, -128.0); /* 0 units */
     const double t = d + 0x1.8p52;
     const double f = d - (t - 0x1.8p52);
-    constexpr double ln2 = 0.69314718055994530942;
-    constexpr double q2 = ln2 * ln2, q4 = q2 * q2, q8 = q4 * q4;
-    double y = q8 * q4 / 479001600.0;
-    y = fma(y, f, q8 * q2 * ln2 / 39916800.0);
-    y = fma(y, f, q8 * q2 / 3628800.0);
-    y = fma(y, f, q8 * ln2 / 362880.0);
-    y = fma(y, f, q8 / 40320.0);
-    y = fma(y, f, q4 * q2 * ln2 / 5040.0);
-    y = fma(y, f, q4 * q2 / 720.0);
-    y = fma(y, f, q4 * ln2 / 120.0);
-    y = fma(y, f, q4 / 24.0);
-    y = fma(y, f, q2 * ln2 / 6.0);
-    y = fma(y, f, q2 / 2.0);
-    y = fma(y, f, ln2);
+    double y = 0x1.e6063f7217bc6p-28;
+    y = fma(y, f, 0x1.b675bca4eeebbp-24);
+    y = fma(y, f, 0x1.62bfd47773353p-20);
+    y = fma(y, f, 0x1.ffcb54062e698p-17);
+    y = fma(y, f, 0x1.430913096fd9fp-13);
+    y = fma(y, f, 0x1.5d87fe9d7a584p-10);
+    y = fma(y, f, 0x1.3b2ab6fba1ddap-7);
+    y = fma(y, f, 0x1.c6b08d703ce49p-5);
+    y = fma(y, f, 0x1.ebfbdff82c598p-3);
+    y = fma(y, f, 0x1.62e42fefa3a19p-1);
     y = fma(y, f, 1.0);
     const int k = (int)(u32)__double_as_longlong(t) + shift;
     return __hiloint2double(__double2hiint(y) + (k << 20), __double2loint(y));
@@ -540,12 +536,15 @@ template <bool kF32, int kLds> struct Row {
   static __device__ __forceinline__ float clean(float l) {
     return l > -INFINITY ? l + 0.0f : -INFINITY;
   }
+  /* kRaw: as they are. */
+  template <bool kRaw = false>
   __device__ __forceinline__ void from_memory(int i, int end, float (&l)[4]) const {
     if (i + 3 < end) {
       const V v = *reinterpret_cast<const V *>(p + (int64_t)i * kSize);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        l[e] = clean(Four<kF32>::value(v[e]));
+        const float x = Four<kF32>::value(v[e]);
+        l[e] = kRaw ? x : clean(x);
       }
       return;
     }
@@ -561,8 +560,9 @@ template <bool kF32, int kLds> struct Row {
       }
     }
   }
+  template <bool kRaw = false>
   __device__ __forceinline__ void load4(int i, int end, float (&l)[4]) const {
-    load(i, end, l);
+    load<kRaw>(i, end, l);
     if (inf) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -570,6 +570,7 @@ template <bool kF32, int kLds> struct Row {
       }
     }
   }
+  template <bool kRaw>
   __device__ __forceinline__ void load(int i, int end, float (&l)[4]) const {
     if constexpr (kLds > 0) {
       if (i >= end) {
@@ -579,10 +580,10 @@ template <bool kF32, int kLds> struct Row {
       const VA v = *(const VX_LDS VA *)(uintptr_t)(lds + (u32)i * kSize);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        l[e] = i + e < end ? clean(Four<kF32>::value(v[e])) : -INFINITY;
+        l[e] = i + e < end ? Four<kF32>::value(v[e]) : -INFINITY; /* clean already */
       }
     } else {
-      from_memory(i, end, l);
+      from_memory<kRaw>(i, end, l);
     }
   }
   /* The first reading: the thread's largest logit, and into LDS. */
@@ -610,14 +611,14 @@ template <bool kF32, int kLds> struct Row {
   }
   /* f(index, logit), in no order. Out of memory four loads a thread are in
    * flight, -inf past the end. */
-  template <typename F> __device__ __forceinline__ void each(F f) const {
+  template <bool kRaw = false, typename F> __device__ __forceinline__ void each(F f) const {
     constexpr int kAhead = kLds > 0 ? 1 : 4;
 #pragma unroll 1
     for (int i = begin + 4 * threadIdx.x; i < end; i += kAhead * kChunk) {
       float v[kAhead][4];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        load4(i + j * kChunk, end, v[j]);
+        load4<kRaw>(i + j * kChunk, end, v[j]);
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
@@ -649,7 +650,7 @@ __device__ __forceinline__ void draw(const SampleArgs &a, Shared &sh, int r, con
       float v[kAhead][4];
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
-        row.load4(i + j * 256, i1, v[j]);
+        row.template load4<W::kRaw>(i + j * 256, i1, v[j]);
       }
 #pragma unroll
       for (int j = 0; j < kAhead; ++j) {
@@ -696,7 +697,7 @@ __device__ __forceinline__ void draw(const SampleArgs &a, Shared &sh, int r, con
     v[e] = -INFINITY;
   }
   if (i < end) {
-    row.load4(i, end, v);
+    row.template load4<W::kRaw>(i, end, v);
   }
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
@@ -766,18 +767,32 @@ __device__ __forceinline__ void finish(const SampleArgs &a, Shared &sh, int r, c
   }
 }
 
-/* A token's weight, where min_p and (kBordered) a border keep it, else 0. */
-template <bool kBordered> struct Keep {
+/* A token's weight, 0 where min_p (kLeast) or a border (kBordered) hides it.
+ * Without a border -0 and NaN need no care: units() makes nothing of either. */
+template <bool kBordered, bool kLeast> struct Keep {
+  static constexpr bool kRaw = !kBordered;
   const Scale &x;
   double least; /* units */
   Border border;
 
   __device__ __forceinline__ u64 operator()(u32 i, float l) const {
     const double q = x.units(l);
-    const u64 w = q >= least ? Scale::whole(q) : u64(0);
+    u64 w = Scale::whole(q);
+    if constexpr (kLeast) {
+      w = q >= least ? w : u64(0);
+    }
     return !kBordered || border.keeps(key_of(l), i) ? w : u64(0);
   }
 };
+/* f(a Keep without a border). */
+template <typename F>
+__device__ __forceinline__ void unbordered(const Scale &x, const Settings &s, F f) {
+  if (s.min_p > 0.0f) {
+    f(Keep<false, true>{x, x.share(s.min_p), {}});
+  } else {
+    f(Keep<false, false>{x, 0.0, {}});
+  }
+}
 
 /* Where the border of top_k, or without it of top_p, lies in the row's histogram,
  * which is in the threads' registers (`mass` only where no top_k is on). */
@@ -813,7 +828,8 @@ __device__ __forceinline__ Where locate(Shared &sh, const Settings &s, u64 mass,
   return w;
 }
 
-/* What is left to do once the row's histogram is known. */
+/* What is left to do once the row's histogram is known (without counts where no
+ * top_k is on). */
 template <typename R>
 __device__ __forceinline__ void finish_bins(const SampleArgs &a, Shared &sh, int r, const R &row, Settings s,
                             const Scale &x, u64 mass, u32 count) {
@@ -838,15 +854,18 @@ __device__ __forceinline__ void finish_bins(const SampleArgs &a, Shared &sh, int
       }
     }
   }
-  if (bordered && at.n <= (u32)kList) {
-    finish(a, sh, r, s, x, gather(sh, row, x, at.bin, sh.list_k), at.sum, at.bin);
-    return;
+  if (bordered && (!s.top_k || at.n <= (u32)kList)) {
+    const int n = gather(sh, row, x, at.bin, sh.list_k);
+    if (n <= kList) {
+      finish(a, sh, r, s, x, n, at.sum, at.bin);
+      return;
+    }
   }
   if (!bordered) {
-    draw(a, sh, r, row, s.u, Keep<false>{x, x.share(s.min_p), {}});
+    unbordered(x, s, [&](auto keep) { draw(a, sh, r, row, s.u, keep); });
     return;
   }
-  Keep<true> keep{x, x.share(s.min_p), {0, 0xffffffffu}};
+  Keep<true, true> keep{x, x.share(s.min_p), {0, 0xffffffffu}};
   {
     /* the border's own bin, then, after top_k, what that keeps */
     bool all = false;
@@ -965,8 +984,9 @@ __global__ __launch_bounds__(kThreads) void sample_rows(SampleArgs a) {
     row.each([&](u32, float l) {
       if (l > -INFINITY) {
         const int b = x.bin(l);
-        atomicAdd(&sh.count[b], 1u);
-        if (!s.top_k) {
+        if (s.top_k) {
+          atomicAdd(&sh.count[b], 1u);
+        } else {
           atomicAdd(&sh.mass[b], x.weight(l));
         }
       }
@@ -1085,9 +1105,10 @@ template <bool kF32> __global__ __launch_bounds__(kThreads) void sample_weigh(Sa
   sh.count[t] = 0;
   __syncthreads();
   if (!s.top_k && s.top_p >= 1.0f) {
-    const Keep<false> keep{x, x.share(s.min_p), {}};
     u64 sum = 0;
-    row.each([&](u32 i, float l) { sum += keep(i, l); });
+    unbordered(x, s, [&](auto keep) {
+      row.template each<true>([&](u32 i, float l) { sum += keep(i, l); });
+    });
     sum = block_sum(sh, sum);
     if (t == 0) {
       shelf->sums(p.slices)[slice] = sum;
@@ -1135,7 +1156,7 @@ __device__ __forceinline__ void finish_slices(const SampleArgs &a, Shared &sh, i
   const u64 want = part_of<true>(s.top_p, at.sum);
   const Point point = descend<true>(sh, by_key, max(key_of(x.least(at.f.bin)), 1u),
                                     key_of(x.ftop), at.f.above_mass, 0, want);
-  const Keep<true> keep{x, 0.0, border_at(sh, both, point, ties_of(point.f, want), a.vocab)};
+  const Keep<true, false> keep{x, 0.0, border_at(sh, both, point, ties_of(point.f, want), a.vocab)};
   /* the kept weight of each slice */
   __syncthreads();
   sh.mass[t] = 0;
@@ -1195,8 +1216,7 @@ template <bool kF32> __global__ __launch_bounds__(kThreads) void sample_settle(S
     const Drawn d = draw_part(sh, t < p.slices ? shelf->sums(p.slices)[t] : 0, s.u);
     mine.begin = d.at * p.slice;
     mine.end = min(mine.begin + p.slice, a.vocab);
-    draw(a, sh, r, mine, s.u, Keep<false>{x, x.share(s.min_p), {}}, d.total,
-         d.target);
+    unbordered(x, s, [&](auto keep) { draw(a, sh, r, mine, s.u, keep, d.total, d.target); });
     return;
   }
   const Where at = locate(sh, s, shelf->mass[t], shelf->count[t]);
@@ -1270,7 +1290,7 @@ template <bool kF32> void launch(const SampleArgs &a, const SamplePlan &plan, ch
 SamplePlan sample_plan(int64_t rows, int64_t vocab, bool borders, bool may_split) {
   SamplePlan p{1, 0, 0};
   const int64_t chunks = (vocab + kChunk - 1) / kChunk;
-  if (!may_split || vocab <= 32768 || rows > (borders ? 4096 : 128)) {
+  if (!may_split || vocab <= 32768 || rows > (borders ? 1024 : 128)) {
     return p;
   }
   /* slices of 1 to 8 chunks, as many as two workgroups a CU of 256 */

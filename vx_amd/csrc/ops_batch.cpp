@@ -157,7 +157,8 @@ int32_t rope_append(const char *op, bool f32, const void *qkv, const float *rope
     return refuse(VX_OP_EUNSUPP, op, "head_dim must be a multiple of 8 and at most 512");
   }
   const int64_t units = product({batch, seq_q, heads + 2 * kv_heads, head_dim / 8});
-  if (units < 0 || units > int64_t(INT32_MAX) * 256 || seq_q > INT32_MAX ||
+  /* a thread a unit: their number is 31-bit */
+  if (units < 0 || units > INT32_MAX || seq_q > INT32_MAX ||
       heads > INT32_MAX / 4 || kv_heads > INT32_MAX / 4 || capacity > INT32_MAX ||
       product({batch, kv_heads, capacity, head_dim}) < 0) {
     return refuse(VX_OP_EUNSUPP, op, "extents past 2^31");
@@ -187,7 +188,7 @@ int32_t sample(const char *op, bool f32, const void *logits, const float *temper
   const int64_t need = vx_nn_sample_workspace(rows, vocab);
   if (need < 0 || stride < vocab || stride > kMaxExtent) {
     return refuse(VX_OP_EINVAL, op,
-                  "rows must be 1..2^31 - 1, vocab 1..2^30 and stride at least vocab");
+                  "rows must be 1..2^21, vocab 1..2^30 and stride at least vocab");
   }
   if (workspace && workspace_bytes < need) {
     return refuse(VX_OP_EINVAL, op, "the workspace is smaller than vx_nn_sample_workspace()");
@@ -322,7 +323,8 @@ int32_t vx_nn_flash_attention_shared_bf16(
 }
 
 int64_t vx_nn_sample_workspace(int64_t rows, int64_t vocab) {
-  if (rows < 1 || rows > INT32_MAX || vocab < 1 || vocab > (int64_t(1) << 30)) {
+  /* 1024 threads a row: their number is 32-bit */
+  if (rows < 1 || rows > (int64_t(1) << 21) || vocab < 1 || vocab > (int64_t(1) << 30)) {
     return VX_OP_EINVAL;
   }
   return vxk::sample_plan(rows, vocab, true, true).ws_bytes;
