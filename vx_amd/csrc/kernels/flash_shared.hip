@@ -1130,10 +1130,17 @@ SharedPlan flash_shared_plan(int64_t batch, int heads, int kv_heads, int seq_q, 
     /* the shared keys once for rows of many sequences */
     const int64_t rows_kv = batch * rows_seq;
     p.shared_rows = p.own_rows && rows_kv <= 16;
-    p.tile = rows_kv <= 64 ? 64 : 128;
+    const int64_t blocks = (shared_len + kBK - 1) / kBK;
+    /* 128 rows where there are as many and their workgroups half fill the CUs:
+     * 33 sequences of 5 queries, 21 heads on 3, over 2047 keys 17 us in tiles
+     * of 64 and 19 of 128, 64 of 8, 32 heads on 8, over 4000 87 and 69 */
+    const int64_t wide = kv_heads * ((rows_kv + 127) / 128);
+    p.tile = rows_kv <= 64 || (!p.own_rows && wide * shared_splits(wide, blocks, cus) < cus / 2)
+                 ? 64
+                 : 128;
     const int tile = p.shared_rows ? 16 : p.tile;
     const int64_t items = kv_heads * ((rows_kv + tile - 1) / tile);
-    p.shared_splits = shared_splits(items, (shared_len + kBK - 1) / kBK, cus);
+    p.shared_splits = shared_splits(items, blocks, cus);
     p.shared_groups = (int)(items * p.shared_splits);
     p.own_splits = capacity > 0 ? 1 : 0;
   }

@@ -84,11 +84,18 @@ struct Settings {
   float u;   /* in [0, 1) */
 };
 __device__ __forceinline__ Settings settings_of(const SampleArgs &a, int r) {
-  const float heat = a.temperature ? a.temperature[r] : 1.0f;
-  const int top_k = a.top_k ? a.top_k[r] : 0;
-  const float top_p = a.top_p ? a.top_p[r] : 1.0f;
-  const float min_p = a.min_p ? a.min_p[r] : 0.0f;
-  const float u = a.u[a.step ? max(*a.step - a.step0, 0) : r];
+  /* one of the pointers is always good to read, so that all loads go together */
+  auto value = [&](const float *p, float none) {
+    const float v = (p ? p : a.u)[p ? r : 0];
+    return p ? v : none;
+  };
+  const int *steps = a.step ? a.step : reinterpret_cast<const int *>(a.u);
+  const int at = steps[0];
+  const float heat = value(a.temperature, 1.0f);
+  const int top_k = __float_as_int(value(reinterpret_cast<const float *>(a.top_k), 0.0f));
+  const float top_p = value(a.top_p, 1.0f);
+  const float min_p = value(a.min_p, 0.0f);
+  const float u = a.u[a.step ? max(at - a.step0, 0) : r];
   Settings s;
   s.u = u > 0.0f ? fminf(u, 0x1.fffffep-1f) : 0.0f;
   s.first = !(heat > 0.0f) || top_k == 1 || top_p <= 0.0f;
