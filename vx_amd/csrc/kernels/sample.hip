@@ -396,12 +396,13 @@ __device__ __forceinline__ void put(const SampleArgs &a, int r, int token, u64 w
 
 /* Everything that is left to do for at most kFew tokens in the list: a token's
  * place in the order, and the weight before it there and by index, by comparing
- * it with each, kSlices threads a token. `mass`: the weight that top_p is a
+ * it with each, 4 to 16 threads a token. `mass`: the weight that top_p is a
  * share of, where no top_k is on. */
 __device__ __forceinline__ void finish_few(const SampleArgs &a, Shared &sh, int r, const Settings &s,
                            const Scale &x, int n, u64 mass) {
-  constexpr int kSlices = kThreads / kFew;
-  const int t = threadIdx.x, e = t % kFew, slice = t / kFew;
+  const int room = n <= 64 ? 64 : n <= 128 ? 128 : kFew;
+  const int slices = kThreads / room;
+  const int t = threadIdx.x, e = t & (room - 1), slice = t / room;
   const bool real = e < n;
   const u64 k = real ? sh.list_k[e] : 0;
   const u32 i = ~(u32)k;
@@ -416,7 +417,7 @@ __device__ __forceinline__ void finish_few(const SampleArgs &a, Shared &sh, int 
     u64 before = 0;
     u32 rank = 0;
 #pragma unroll 4
-    for (int j = slice; j < n; j += kSlices) {
+    for (int j = slice; j < n; j += slices) {
       const bool over = sh.list_k[j] > k;
       rank += over ? 1u : 0u;
       before += over ? sh.list_w[j] : 0;
@@ -447,7 +448,7 @@ __device__ __forceinline__ void finish_few(const SampleArgs &a, Shared &sh, int 
   if (real) {
     u64 before = 0;
 #pragma unroll 4
-    for (int j = slice; j < n; j += kSlices) {
+    for (int j = slice; j < n; j += slices) {
       before += ~(u32)sh.list_k[j] < i ? sh.list_w[j] : 0;
     }
     atomicAdd(&sh.mass[kFew + e], before);
@@ -596,7 +597,7 @@ template <bool kF32, int kLds> struct Row {
   /* The first reading: the thread's largest logit, and into LDS. */
   __device__ __forceinline__ float take() const {
     float top = -INFINITY;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = begin + 4 * threadIdx.x; i < end; i += kChunk) {
       float l[4];
       from_memory(i, end, l);
@@ -873,7 +874,23 @@ __device__ __forceinline__ void finish_bins(const SampleArgs &a, Shared &sh, int
     return;
   }
   Keep<true, true> keep{x, x.share(s.min_p), {0, 0xffffffffu}};
-  {
+  const u32 lo = max(key_of(x.least(at.f.bin)), 1u), hi = key_of(x.ftop);
+  const int in_bin = s.top_k ? kList + 1 : gather<true>(sh, row, x, at.f.bin, sh.list_k);
+  if (in_bin <= kList) {
+    /* the border's bin alone, in the list */
+    const bool mine = t < in_bin;
+    const u64 kw = mine ? sh.list_k[t] : 0;
+    const u64 w = mine ? x.weight(logit_of((u32)(kw >> 32))) : 0;
+    auto both = [&](auto take) {
+      if (mine) {
+        take((u32)(kw >> 32), ~(u32)kw, [&] { return w; });
+      }
+    };
+    auto by_key = [&](auto take) { both([&](u32 key, u32, auto weight) { take(key, weight); }); };
+    const u64 want = part_of<true>(s.top_p, at.sum);
+    const Point p = descend<true>(sh, by_key, lo, hi, at.f.above_mass, 0, want);
+    keep.border = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
+  } else {
     /* the border's own bin, then, after top_k, what that keeps */
     bool all = false;
     auto passes = [&](u32 k, u32 i, float l) {
@@ -895,7 +912,6 @@ __device__ __forceinline__ void finish_bins(const SampleArgs &a, Shared &sh, int
         }
       });
     };
-    const u32 lo = max(key_of(x.least(at.f.bin)), 1u), hi = key_of(x.ftop);
     if (s.top_k) {
       const Point p =
           descend<false>(sh, by_key, lo, hi, 0, at.f.above_count, (u64)s.top_k);
