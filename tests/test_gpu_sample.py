@@ -282,6 +282,24 @@ def test_wide_borders(hiplib, vocab, dtype):
         check(hiplib, x, u, dtype=dtype, **kw)
 
 
+@pytest.mark.parametrize("vocab", [6000, 70000])
+@pytest.mark.parametrize("kept", [30, 200, 300, 900, 1500])
+def test_min_p_before_the_other_border(hiplib, vocab, kept):
+    """min_p keeps `kept` tokens, of which top_k and top_p would each keep all and
+    more."""
+    announce(f"sample min_p keeps {kept} of {vocab}")
+    rng = np.random.default_rng([vocab, kept])
+    rows = 6
+    x = (-4 - 0.5 * rng.random((rows, vocab))).astype(np.float32)
+    for r in range(rows):
+        x[r, rng.choice(vocab, kept, replace=False)] = 2 * rng.random(kept, dtype=np.float32)
+        x[r, rng.integers(vocab)] = 2
+    u = rng.random(rows, dtype=np.float32)
+    for kw in (dict(top_k=kept + 700), dict(top_k=kept + 2), dict(top_p=0.9999), dict(top_p=0.97),
+               dict(top_k=kept + 1000, top_p=0.9999)):
+        check(hiplib, x, u, min_p=0.1, **kw)
+
+
 def test_two_streams_at_once(hiplib):
     announce("sample on two streams")
     t = HipTimer()

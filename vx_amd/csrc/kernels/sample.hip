@@ -462,7 +462,8 @@ __device__ __forceinline__ void finish_few(const SampleArgs &a, Shared &sh, int 
   }
 }
 
-/* The same for up to kList tokens, one a thread, of bins up to `bin`. */
+/* The same for up to kList tokens, one a thread, of bins up to `bin`. Where min_p
+ * leaves no more than those, the border of top_k or top_p may lie below them all. */
 __device__ __forceinline__ void finish_list(const SampleArgs &a, Shared &sh, int r, const Settings &s,
                             const Scale &x, int n, u64 mass, int bin) {
   const int t = threadIdx.x;
@@ -484,16 +485,20 @@ __device__ __forceinline__ void finish_list(const SampleArgs &a, Shared &sh, int
     }
   };
   if (s.top_k) {
-    const Point p = descend<false>(sh, by_key, lo, hi, 0, 0, (u64)s.top_k);
-    const Border b = border_at(sh, both, p, (u64)s.top_k - p.f.above_count, a.vocab);
-    in = mine && b.keeps(key, i);
+    if (s.top_k < n) {
+      const Point p = descend<false>(sh, by_key, lo, hi, 0, 0, (u64)s.top_k);
+      const Border b = border_at(sh, both, p, (u64)s.top_k - p.f.above_count, a.vocab);
+      in = mine && b.keeps(key, i);
+    }
     mass = s.top_p < 1.0f ? block_sum(sh, in ? w : 0) : 0;
   }
   if (s.top_p < 1.0f) {
     const u64 want = part_of<true>(s.top_p, mass);
-    const Point p = descend<true>(sh, by_key, lo, hi, 0, 0, want);
-    const Border b = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
-    in = in && b.keeps(key, i);
+    if (want <= block_sum(sh, in ? w : 0)) {
+      const Point p = descend<true>(sh, by_key, lo, hi, 0, 0, want);
+      const Border b = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
+      in = in && b.keeps(key, i);
+    }
   }
   if (s.min_p > 0.0f) {
     in = in && x.units(logit_of(key)) >= x.share(s.min_p);
@@ -853,7 +858,7 @@ __device__ __forceinline__ void finish_bins(const SampleArgs &a, Shared &sh, int
         sh.mass[t] = 0;
         __syncthreads();
         row.each([&](u32, float l) {
-            if (l > -INFINITY) {
+          if (l > -INFINITY) {
             atomicAdd(&sh.mass[x.bin(l)], x.weight(l));
           }
         });
