@@ -300,6 +300,22 @@ def test_min_p_before_the_other_border(hiplib, vocab, kept):
         check(hiplib, x, u, min_p=0.1, **kw)
 
 
+@pytest.mark.parametrize("vocab", [1200, 9000, 70000])
+def test_top_p_within_what_top_k_keeps_of_equals(hiplib, vocab):
+    """top_k ends among many equal logits, and top_p keeps nearly or quite all that
+    it leaves."""
+    announce(f"sample equals by top_k and top_p {vocab}")
+    rng = np.random.default_rng(vocab)
+    x = np.zeros((8, vocab), np.float32)
+    x[4:, ::3] = 0.5
+    u = rng.random(8, dtype=np.float32)
+    for k in (2, 22, vocab // 3, vocab - 7):
+        want = check(hiplib, x, u, top_k=k, top_p=1 - 2.0 ** -20)
+        assert np.all(want[0][:4] < k)
+        check(hiplib, x, u, top_k=k, top_p=0.999)
+        check(hiplib, x, u, top_k=k, top_p=0.6, dtype="bf16")
+
+
 def test_two_streams_at_once(hiplib):
     announce("sample on two streams")
     t = HipTimer()

@@ -932,7 +932,9 @@ __device__ __forceinline__ void finish_bins(const SampleArgs &a, Shared &sh, int
     if (s.top_p < 1.0f) {
       const u64 want = part_of<true>(s.top_p, at.sum);
       const Point p = descend<true>(sh, by_key, lo, hi, at.f.above_mass, 0, want);
-      keep.border = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
+      const Border b = border_at(sh, both, p, ties_of(p.f, want), a.vocab);
+      /* of equal logits top_k may have kept fewer than there are */
+      keep.border = Border{b.key, b.key == keep.border.key ? min(b.last, keep.border.last) : b.last};
     }
   }
   draw(a, sh, r, row, s.u, keep);
