@@ -148,7 +148,8 @@ int32_t vx_nn_rope_append_f32(const float *qkv, const float *rope,
  * shared_len + lens[b]. A key that a query does not see does not reach its
  * result, whatever its values; a query that sees none gets o = 0 and lse =
  * -inf. k_shared and v_shared may be NULL where shared_len is 0, k and v
- * where capacity is 0. head_dim 64 or 128; pointers 16-byte aligned. */
+ * where capacity is 0. head_dim 64 or 128; pointers 16-byte aligned; scale and
+ * scale * log2(e) finite. */
 int32_t vx_nn_flash_attention_shared_bf16(
     const uint16_t *q, const uint16_t *k_shared, const uint16_t *v_shared,
     const uint16_t *k, const uint16_t *v, const int32_t *lens, uint16_t *o,

@@ -85,6 +85,11 @@ def test_shared_attention_refuses(lib, p, kw, code):
     assert shared(lib, p, **kw) == code
 
 
+@pytest.mark.parametrize("scale", [3e38, -3e38])
+def test_shared_attention_refuses_a_scale_past_base_2(lib, p, scale):
+    assert shared(lib, p, scale=scale) == EINVAL
+
+
 def test_shared_attention_refuses_alignment(lib, p):
     for name in ("q", "k_shared", "v_shared", "k", "v", "o"):
         assert shared(lib, p, **{name: p + 8}) == EUNSUPP, name

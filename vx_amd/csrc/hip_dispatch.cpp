@@ -140,9 +140,8 @@ void select_device(int32_t topology_id, const char *why) {
   }
 }
 
-/* True for memory the GPU owns (hipMalloc'd). Host memory, registered or not,
- * answers false. */
-/* The GPU whose memory `p` is, -1 where it is not GPU memory. */
+/* The GPU whose memory (hipMalloc'd) `p` is, -1 where it is not GPU memory.
+ * Host memory, registered or not, is not. */
 int device_of_ptr(const void *p) {
   if (!p || !hip_available()) {
     return -1;

@@ -287,8 +287,8 @@ int32_t vx_nn_flash_attention_shared_bf16(
     return refuse(VX_OP_EINVAL, op, "q, o and the keys and values of what is not empty must not "
                                     "be NULL");
   }
-  if (!std::isfinite(scale)) {
-    return refuse(VX_OP_EINVAL, op, "scale must be finite");
+  if (!std::isfinite(scale * 1.4426950408889634f)) { /* the exponentials are of base 2 */
+    return refuse(VX_OP_EINVAL, op, "scale must be finite, and times log2(e) too");
   }
   if (shared_capacity < shared_len || shared_capacity > INT32_MAX / 256) {
     return refuse(VX_OP_EINVAL, op, "shared_capacity must be at least shared_len and below 2^23");
