@@ -1,6 +1,6 @@
 /*
  * decode.cpp -- vx_llama_i8_*: an int8 Llama-2-style decoder resident in HBM
- * and its greedy generation loop (include/vx_hip_ops.h).
+ * and its generation loops, greedy and sampled (include/vx_hip_ops.h).
  *
  * Weights are re-laid out once at upload so each fused kernel streams one
  * matrix: per layer [Wq; Wk; Wv] stacked (one GEMV feeds RoPE and the KV
@@ -11,7 +11,9 @@
  * launches that, with VX_LLAMA_GRAPH, is captured into hipGraphs of
  * kGraphSteps steps and of one step (kept with the model while the prompt
  * length and I/O buffers stay the same) and replayed with no host
- * synchronisation until the tokens are read back.
+ * synchronisation until the tokens are read back. A sampled step has the
+ * draw's launches after those (kernels/sample.hip; one up to a vocabulary of
+ * 32768, else three), with graphs of its own.
  */
 #include "../../include/vx_hardware_runtime.h"
 #include "../../include/vx_hip_ops.h"

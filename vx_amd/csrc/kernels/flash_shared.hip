@@ -24,6 +24,13 @@
  * A block in which a key is hidden from one of a wave's queries and not from
  * another goes a key at a time where V there holds infinities or NaNs (0 x inf
  * is NaN), each key for the queries that see it.
+ *
+ * 16 sequences, 32 heads on 8 of 128, over 65536 shared and 128 own keys: 58 us
+ * for 298 MB of keys, 5.1 TB/s, and 5 for the merge: the keys' bytes bound it. 64
+ * on 4 KV heads over 8192: 25 and 5.3, where 10 would read the keys and 7 multiply;
+ * a workgroup of 128 rows spends 8 us of its 25 before its first and after its
+ * last block of 64 keys, and 1.7 on each. 8 sequences of 256 queries, 32 heads on
+ * 8, over 4096 and 300 own, causal: 176 us, 810 TFLOP/s.
  */
 #include "../vx_batch_kernels.h"
 #include "../vx_hip_common.h"
@@ -107,8 +114,8 @@ __device__ __forceinline__ Row row_of(const KernelArgs &p, int kv, int b, int r)
 }
 
 /* Eight elements of a row's query, from column c on; of a row that is none they
- * stay in its own column of every product. The scale's sign goes into the query, so that a hidden key's score is
- * -inf whatever the scale. */
+ * stay in its own column of every product. The scale's sign goes into the query,
+ * so that a hidden key's score is -inf whatever the scale. */
 __device__ __forceinline__ u32x4 query(const KernelArgs &p, const Row &row, int head_dim, int c) {
   u32x4 q = {0, 0, 0, 0};
   if (row.place >= 0) {

@@ -6,6 +6,9 @@
  * rounded to bf16 once. Bound by memory: each element of the projection is
  * read once and written once, the table's rows come from L2 after their first
  * head. A thread takes 8 elements, 16 bytes of output and 32 of the table.
+ *
+ * 8 sequences x 256 tokens, 32 heads on 8, head_dim 128: 51 MB in 10.9 us, 4.7
+ * TB/s, the rate of a large copy. 4 x 1, 12 heads of 64: 2.9 us, a launch.
  */
 #include "../vx_batch_kernels.h"
 #include "../vx_hip_common.h"
