@@ -29,8 +29,8 @@
  * Latency bounds the small calls. 1 x 32000 f32 by top-k and top-p 10.1 us: 4.1
  * for the row's 128 KB into LDS by one workgroup, 1.5 for the maxima and their
  * bin, 3.1 for the list, 3.3 for the rest; 48 x 32000 with every setting in use
- * 22.8, of which the 64-bit weights of rows with top-p alone, 32 a thread and an
- * LDS atomic each, take 11. 8 x 131072 by top-p 23.5 in three launches (3.1, 7.4,
+ * 22.8, of which the 64-bit weights of rows with top-p alone, 32 a thread, take
+ * 11 (atomics for the tokens near the border alone save nothing). 8 x 131072 by top-p 23.5 in three launches (3.1, 7.4,
  * 13.0). 256 x 131071 without a border 64: the row out of memory twice, 269 MB at
  * 4.2 TB/s, and 512 64-bit weights a thread, 33 us on one CU.
  */
