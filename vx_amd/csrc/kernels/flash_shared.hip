@@ -271,8 +271,8 @@ __device__ __forceinline__ void wide(const KernelArgs &p, const Item &it, char *
       rs[w] = __builtin_amdgcn_readfirstlane(rs[w]); /* uniform, which the compiler cannot tell */
     }
     const uint32_t base = ring_base + (uint32_t)((((j & 1) * 2 + plane) * kUnits + wq * 64) * 16);
-    const int tg = wq * 64 + lane_here();
-    const int row = tg / kChunks, c = tg % kChunks;
+    const uint32_t tg = (uint32_t)(wq * 64 + lane_here());
+    const int row = (int)(tg / kChunks), c = (int)(tg % kChunks);
     const int off =
         row * kRowBytes + (plane == 0 ? place_k<kChunks>(row, c) : place_v<kChunks>(row, c)) * 16;
 #pragma unroll
