@@ -36,6 +36,7 @@
  */
 #include "../vx_batch_kernels.h"
 #include "../vx_hip_common.h"
+#include "sample_list.h"
 #include "vx_lds_dma.hip.h"
 #include "vx_wave_ops.hip.h"
 
@@ -748,29 +749,29 @@ __device__ __forceinline__ void draw(const SampleArgs &a, Shared &sh, int r, con
   }
 }
 
+/* A workgroup's threads, for fill_list. */
+struct Group {
+  __device__ __forceinline__ int thread() const { return (int)threadIdx.x; }
+  __device__ __forceinline__ void sync() const { __syncthreads(); }
+  __device__ __forceinline__ u32 add(u32 &n) const { return atomicAdd(&n, 1u); }
+};
+
 /* The row's tokens of bins up to `bin` (kOne: of that bin) into the list; how
  * many there are, of which it holds the first kCap. */
 template <bool kOne = false, int kCap, typename R>
 __device__ __forceinline__ int gather(Shared &sh, const R &row, const Scale &x, int bin,
                                       u64 (&list)[kCap]) {
-  if (threadIdx.x == 0) {
-    sh.n = 0;
-  }
-  __syncthreads();
   const float least = x.least(bin);
-  row.each([&](u32 i, float l) {
-    if (l >= least) { /* one of a few, mostly */
-      const int b = x.bin(l);
-      if (l > -INFINITY && (kOne ? b == bin : b <= bin)) {
-        const u32 at = atomicAdd(&sh.n, 1u);
-        if (at < (u32)kCap) {
-          list[at] = (u64)key_of(l) << 32 | (u32)~i;
+  return fill_list(Group{}, sh.n, list, [&](auto take) {
+    row.each([&](u32 i, float l) {
+      if (l >= least) { /* one of a few, mostly */
+        const int b = x.bin(l);
+        if (l > -INFINITY && (kOne ? b == bin : b <= bin)) {
+          take((u64)key_of(l) << 32 | (u32)~i);
         }
       }
-    }
+    });
   });
-  __syncthreads();
-  return (int)sh.n;
 }
 
 /* The result from the list's n tokens, those of bins up to `bin`. */
