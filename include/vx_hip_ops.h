@@ -105,7 +105,8 @@ int32_t vx_nn_gemv_i8_bf16(const int8_t *w, const float *scale,
  * work is given one of at least *_workspace() bytes (a smaller one is refused),
  * which two launches that may run at the same time must not share. Sampling
  * uses at most 1024 x (45 KiB + 8.2 KiB per 32768 logits), attention 4 *
- * (head_dim + 2) bytes a query of a head for each part of the keys. */
+ * (head_dim + 2) bytes a query of a head for each part of the keys (of each
+ * part up to 8 more). */
 
 /* Splits, rotates and appends. qkv: [batch, seq_q, heads + 2 * kv_heads,
  * head_dim] (a token's queries, keys and values together, as one projection

@@ -113,6 +113,19 @@ def test_shared_attention_workspace(lib, p):
             assert shared(lib, p, workspace=p, workspace_bytes=n - 1, **kw) == EINVAL
 
 
+@pytest.mark.parametrize("ext", [(33, 21, 3, 5, 2047, 333, 64), (33, 21, 3, 5, 2047, 333, 128), (65, 3, 3, 1, 2100, 9, 64),
+                                 (5, 5, 1, 1, 4000, 30, 128), (1, 7, 7, 1, 3000, 200, 64)])
+def test_shared_attention_parts_are_aligned(lib, ext):
+    """Parts of an odd number of rows, 8 bytes past a multiple of 16 each, begin
+    on 16 bytes all the same."""
+    b, h, kv, n, p, cap, d = ext
+    rows = b * h * n
+    assert rows % 2 == 1
+    size = lib.lib.vx_nn_flash_attention_shared_workspace(*ext)
+    part = (rows * (d + 2) * 4 + 15) // 16 * 16
+    assert size >= 2 * part and size % part == 0
+
+
 def draw(lib, p, **kw):
     a = dict(dtype="f32", logits=p, temperature=p, top_k=p, top_p=p, min_p=p, u=p, tokens=p,
              logprob=p, rows=4, vocab=100)

@@ -360,3 +360,16 @@ def test_a_streams_workspace_goes_with_it(hiplib):
     c.check()
     c.free()
     t.stream_destroy(stream)
+
+
+@pytest.mark.parametrize("case", [
+    (33, 21, 3, 5, 2047, 60, 64, [(7 * i) % 56 + 5 for i in range(33)]),
+    (33, 3, 3, 1, 2100, 9, 128, [i % 10 for i in range(33)]),
+    (5, 5, 1, 1, 4000, 30, 128, [1, 30, 0, -1, 17]),
+    (1, 7, 7, 1, 3000, 200, 64, [177])])
+def test_odd_rows_in_parts(hiplib, case):
+    """An odd number of queries in all, several parts of the keys."""
+    announce(f"flash_shared odd rows {case[:7]}")
+    assert case[0] * case[1] * case[3] % 2 == 1
+    assert hiplib.lib.vx_nn_flash_attention_shared_workspace(*case[:7]) > 0
+    both(hiplib, *case)

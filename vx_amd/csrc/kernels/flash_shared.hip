@@ -69,9 +69,12 @@ struct KernelArgs {
 };
 
 /* The workspace's part `part`: [rows][kD] sums, then [rows] statistics (max in
- * base 2, weight). */
+ * base 2, weight). Parts begin on 16 bytes, as their loads and stores do. */
+__host__ __device__ constexpr int64_t part_floats(int64_t rows, int head_dim) {
+  return (rows * (head_dim + 2) + 3) & ~int64_t(3);
+}
 template <int kD> __device__ __forceinline__ float *part_of(const KernelArgs &p, int part) {
-  return reinterpret_cast<float *>(p.ws) + part * (int64_t)p.p.rows * (kD + 2);
+  return reinterpret_cast<float *>(p.ws) + part * part_floats(p.p.rows, kD);
 }
 
 struct Segment {
@@ -1171,7 +1174,7 @@ SharedPlan flash_shared_plan(int64_t batch, int heads, int kv_heads, int seq_q, 
   }
   p.own_groups = (int)(items * p.own_splits);
   p.parts = p.shared_splits + p.own_splits;
-  p.ws_bytes = p.parts > 1 ? (int64_t)p.parts * p.rows * (head_dim + 2) * 4 : 0;
+  p.ws_bytes = p.parts > 1 ? p.parts * part_floats(p.rows, head_dim) * 4 : 0;
   return p;
 }
 
