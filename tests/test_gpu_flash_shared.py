@@ -373,3 +373,37 @@ def test_odd_rows_in_parts(hiplib, case):
     assert case[0] * case[1] * case[3] % 2 == 1
     assert hiplib.lib.vx_nn_flash_attention_shared_workspace(*case[:7]) > 0
     both(hiplib, *case)
+
+
+def test_a_large_workspace_is_not_kept(hiplib):
+    """A call whose parts take more than the library keeps for a stream has them
+    for itself: what is held stays within the limit, here and on the default
+    stream, and smaller calls before and after keep their block."""
+    announce("flash_shared large workspace")
+    limit = 128 << 20
+    lens = [i % 3 if i % 61 == 0 else -1 for i in range(4096)]
+    large = Call(hiplib, 4096, 32, 1, 1, 130, 2, 128, lens, lse=False)
+    small = Call(hiplib, 64, 8, 2, 1, 1500, 40, 128, [i % 41 for i in range(64)])
+    assert large.workspace_bytes() > limit > small.workspace_bytes() > 0
+    wants = large.want(), small.want()
+    t = HipTimer()
+    stream = t.stream_create()
+    try:
+        for s in (stream, None):
+            hiplib.lib.vx_hip_set_stream(s)
+            small()
+            before = held(hiplib)
+            for _ in range(2):
+                large()
+                small()
+                assert held(hiplib) == before
+            assert before[1] <= 2 * limit
+            t.sync()
+            large.check(wants[0])
+            small.check(wants[1])
+    finally:
+        hiplib.lib.vx_hip_set_stream(None)
+        t.sync()
+        large.free()
+        small.free()
+        t.stream_destroy(stream)

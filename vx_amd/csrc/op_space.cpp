@@ -39,17 +39,29 @@ char *op_space(size_t bytes, hipStream_t stream) {
   if (b->base && bytes <= b->bytes) {
     return b->base;
   }
-  void *fresh = nullptr;
-  if (hipMallocAsync(&fresh, bytes, stream) != hipSuccess || !fresh) {
-    (void)hipGetLastError();
+  char *fresh = op_space_once(bytes, stream);
+  if (!fresh) {
     return nullptr;
   }
   if (b->base) {
     VX_HIP_CHECK(hipFreeAsync(b->base, stream));
   }
-  b->base = static_cast<char *>(fresh);
+  b->base = fresh;
   b->bytes = bytes;
   return b->base;
+}
+
+char *op_space_once(size_t bytes, hipStream_t stream) {
+  void *fresh = nullptr;
+  if (hipMallocAsync(&fresh, bytes, stream) != hipSuccess) {
+    (void)hipGetLastError();
+    return nullptr;
+  }
+  return static_cast<char *>(fresh);
+}
+
+void op_space_once_free(char *base, hipStream_t stream) {
+  VX_HIP_CHECK(hipFreeAsync(base, stream));
 }
 
 int op_space_release_stream(hipStream_t stream) {

@@ -94,9 +94,9 @@ private:
   bool moved_ = false;
 };
 
-/* A launch's workspace: the caller's, or the one kept for the stream, held
- * through the scope. A stream that is capturing a graph, or a handle of
- * several streams, has none of the library's. */
+/* A launch's workspace: the caller's, or the one kept for the stream, or (more
+ * than is kept) one for this call, held through the scope. A stream that is
+ * capturing a graph, or a handle of several streams, has none of the library's. */
 class Space {
 public:
   Space(void *given, int64_t bytes) {
@@ -104,16 +104,29 @@ public:
       base = static_cast<char *>(given);
       enough = true;
     } else if (vxk::one_stream(vxops::stream()) && !vxops::capturing()) {
-      hold_ = vxk::op_space_lock();
-      base = vxk::op_space((size_t)bytes, vxops::stream());
+      once_ = bytes > vxk::kOpSpaceKept;
+      if (once_) {
+        base = vxk::op_space_once((size_t)bytes, vxops::stream());
+      } else {
+        hold_ = vxk::op_space_lock();
+        base = vxk::op_space((size_t)bytes, vxops::stream());
+      }
       enough = base != nullptr;
     }
   }
+  ~Space() {
+    if (once_ && base) {
+      vxk::op_space_once_free(base, vxops::stream());
+    }
+  }
+  Space(const Space &) = delete;
+  Space &operator=(const Space &) = delete;
 
   char *base = nullptr;
   bool enough = false;
 
 private:
+  bool once_ = false;
   std::unique_lock<std::mutex> hold_;
 };
 
