@@ -106,7 +106,7 @@ int32_t vx_nn_gemv_i8_bf16(const int8_t *w, const float *scale,
  * workgroup draws each row). A captured call that shall divide its
  * work is given one of at least *_workspace() bytes (a smaller one is refused),
  * which two launches that may run at the same time must not share. Sampling
- * uses at most 1024 x (45 KiB + 8.2 KiB per 32768 logits), attention 4 *
+ * uses at most 1024 x (45 KiB + 8.2 KiB per begun 32768 logits), attention 4 *
  * (head_dim + 2) bytes a query of a head for each part of the keys (of each
  * part up to 8 more). */
 

@@ -160,3 +160,15 @@ def test_sample_workspace(lib, p):
         assert n >= 0
         if n:
             assert draw(lib, p, rows=rows, vocab=vocab, workspace=p, workspace_bytes=n - 1) == EINVAL
+
+
+def test_sample_workspace_stays_within_what_is_said(lib):
+    """1024 x (45 KiB + 8.2 KiB per begun 32768 logits), also just past a multiple."""
+    size = lib.lib.vx_nn_sample_workspace
+    for vocab in (32768, 32769, 33000, 36865, 50000, 65536, 65537, 98305, 131071, 131073, 262144, 262145,
+                  2 ** 25 - 1, 2 ** 25, 2 ** 25 + 1):
+        bound = 1024 * (45 * 1024 + 8.2 * 1024 * -(-vocab // 32768))
+        for rows in (1, 2, 7, 15, 16, 56, 57, 63, 113, 114, 255, 256, 511, 512, 1000, 1023, 1024, 1025):
+            assert 0 <= size(rows, vocab) <= bound, (rows, vocab)
+    # without the rounding up it takes more
+    assert size(1024, 33000) > 1024 * (45 * 1024 + 8.2 * 1024 * 33000 / 32768)
