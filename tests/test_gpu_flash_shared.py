@@ -407,3 +407,79 @@ def test_a_large_workspace_is_not_kept(hiplib):
         large.free()
         small.free()
         t.stream_destroy(stream)
+
+
+# batch, heads, kv_heads, seq_q, shared_len, capacity; lens; and how the call is
+# divided: one tile walks shared and own keys, 16-row tiles of shared and of own
+# keys, rows of a wide tile, workgroups that divide a tile's shared and own keys
+# (tests/test_batch_plans.py holds the rules to it)
+PLANNED = [
+    ((1, 2, 1, 1, 1500, 700), [699], (1, 0, 1, 64, 0, 2)),
+    ((1, 2, 2, 3, 9000, 300), [300], (1, 0, 1, 64, 0, 9)),
+    ((3, 8, 2, 5, 200, 60), [60, 5, 33], (1, 0, 0, 64, 0, 1)),
+    ((1, 4, 1, 6, 3000, 1300), [1201], (1, 0, 0, 64, 0, 8)),
+    ((1, 8, 1, 5, 5100, 70), [70], (1, 0, 0, 64, 0, 10)),
+    ((2, 4, 1, 40, 200, 900), [900, 41], (1, 0, 0, 128, 0, 2)),
+    ((1, 4, 1, 30, 5000, 100), [87], (1, 0, 0, 128, 0, 9)),
+    ((4, 12, 12, 1, 1000, 64), [64, 1, 0, 33], (0, 1, 1, 64, 4, 1)),
+    ((16, 8, 8, 1, 4096, 256), [(19 * i) % 257 for i in range(16)], (0, 1, 1, 64, 16, 1)),
+    ((3, 4, 2, 1, 1300, 1030), [1030, 600, -1], (0, 1, 1, 64, 5, 2)),
+    ((4, 4, 2, 8, 700, 12), [12, 3, 8, 9], (0, 0, 1, 64, 2, 1)),
+    ((8, 32, 8, 1, 3000, 1100), [(157 * i) % 1101 for i in range(8)], (0, 0, 1, 64, 11, 2)),
+    ((16, 4, 2, 8, 700, 12), [i % 13 for i in range(16)], (0, 0, 1, 128, 2, 1)),
+    ((20, 8, 1, 1, 1100, 1030), [1030 if i == 3 else 51 * i for i in range(20)], (0, 0, 1, 128, 4, 2)),
+    ((64, 8, 2, 1, 4600, 40), [i % 41 if i % 4 else -1 for i in range(64)], (0, 0, 1, 128, 18, 1)),
+    ((33, 21, 3, 5, 2047, 90), [(7 * i) % 86 + 5 if i % 3 else -1 for i in range(33)], (0, 0, 0, 64, 4, 1)),
+    ((12, 16, 1, 2, 4000, 1100), [1100, 2, 0, 600] + [40] * 8, (0, 0, 0, 64, 15, 2)),
+    ((64, 32, 8, 8, 600, 20), [i % 21 if i % 4 == 0 else -1 for i in range(64)], (0, 0, 0, 128, 1, 1)),
+    ((32, 64, 2, 2, 4200, 1030), [1030 if i == 8 else 31 * i if i % 4 == 0 else -1 for i in range(32)],
+     (0, 0, 0, 128, 8, 2)),
+]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("case", PLANNED, ids=lambda c: "-".join(map(str, c[0])))
+def test_each_way_of_dividing(hiplib, case, head_dim, causal):
+    announce(f"flash_shared divided {case[0]} {head_dim} causal {causal}")
+    both(hiplib, *case[0], head_dim, case[1], causal=causal, extra=case[0][4] % 2)
+
+
+# fewer own keys than queries, tiles of shared keys alone: 16 rows, 64 and 128
+# rows with 16-row tiles of own keys and without
+SHORT = [((2, 2, 2, 8, 700, 12), (0, 1, 1, 64, 2, 1)), ((4, 4, 2, 8, 700, 12), (0, 0, 1, 64, 2, 1)),
+         ((16, 4, 2, 8, 700, 12), (0, 0, 1, 128, 2, 1)), ((3, 4, 2, 20, 1000, 30), (0, 0, 0, 64, 4, 1)),
+         ((64, 32, 8, 8, 600, 20), (0, 0, 0, 128, 1, 1))]
+
+
+@pytest.mark.parametrize("value", [NAN, INF, 0xFF80, 0x7F7F])
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("case", SHORT, ids=lambda c: "-".join(map(str, c[0])))
+def test_hidden_shared_keys_do_not_reach_a_query(hiplib, case, head_dim, value):
+    """The last three shared keys are NaN, infinities or the largest number: a
+    query that ends before them gets its result all the same, and one that sees
+    them gets NaN where they are NaN."""
+    announce(f"flash_shared hidden shared {case[0]} {head_dim} {value:#x}")
+    b, h, kv, n, p, cap = case[0]
+    # few sequences, so that the plain result is quick
+    lens = [s % n if s % (b // 4 + 1) == 0 or b < 17 else -1 for s in range(b)]
+    clean = Call(hiplib, *case[0], head_dim, lens)
+    (wo, wl), (to, tl) = clean.want()
+    clean.free()
+    last = np.array([[p + m - n + i for i in range(n)] for m in lens])
+    before = np.broadcast_to(((last < p - 3) & (np.array(lens) >= 0)[:, None])[:, None], (b, h, n))
+    after = np.broadcast_to(((last >= p - 1) & (np.array(lens) >= 0)[:, None])[:, None], (b, h, n))
+    assert before.any() and after.any()
+    for name in ("ks", "vs"):
+        c = Call(hiplib, *case[0], head_dim, lens)
+        getattr(c, name)[:, p - 3:p] = value
+        c.d[name].free()
+        c.d[name] = DeviceArray.of(hiplib, getattr(c, name), abi.DTYPE_BF16)
+        c()
+        o, lse = c.results()
+        o = bf16_to_f32(o[:c.q.size]).astype(np.float64).reshape(wo.shape)
+        lse = lse[:b * h * n].astype(np.float64).reshape(wl.shape)
+        assert np.all(np.abs(o - wo)[before] <= to[before]), name
+        assert np.all(np.abs(lse - wl)[before] <= tl[before]), name
+        assert value != NAN or np.all(np.isnan(o[after])), name
+        c.free()

@@ -6,6 +6,8 @@
 #ifndef VX_AMD_BATCH_KERNELS_H
 #define VX_AMD_BATCH_KERNELS_H
 
+#include "kernels/flash_shared.h"
+
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -36,23 +38,6 @@ struct SharedAttnArgs {
   float scale;
   bool causal;
 };
-/* How a call is divided: `shared_groups` workgroups over the shared keys of
- * all sequences' queries, `own_groups` over own keys (`together`: over shared
- * and own ones), parts merged from `ws_bytes` of workspace. */
-struct SharedPlan {
-  int rows;        /* queries of all heads */
-  int parts;       /* partial results of each (1: none, the result itself) */
-  int shared_splits, own_splits; /* workgroups that divide a tile's keys */
-  int shared_groups, own_groups;
-  int own_tiles;   /* tiles of a sequence's queries of a KV head */
-  int tile;        /* rows of a wide tile: 64 or 128 */
-  bool together;
-  bool shared_rows, own_rows; /* 16-row tiles */
-  int64_t ws_bytes;
-};
-/* Plain host arithmetic; `may_split` false: a plan without a workspace. */
-SharedPlan flash_shared_plan(int64_t batch, int heads, int kv_heads, int seq_q, int shared_len,
-                             int capacity, int head_dim, int cus, bool may_split);
 void flash_shared_launch(const SharedAttnArgs &a, const SharedPlan &plan, int head_dim, char *ws,
                          hipStream_t stream);
 
