@@ -105,3 +105,52 @@ def test_refusals(model, hiplib):
     assert fn(model.handle, prompt.ctypes.data, 3, 4, None, u.ctypes.data, toks.ctypes.data, None, 0) == -1
     assert fn(model.handle, prompt.ctypes.data, 3, 4, how.ctypes.data, None, toks.ctypes.data, None, 0) == -1
     assert fn(model.handle, prompt.ctypes.data, 3, 4, how.ctypes.data, u.ctypes.data, toks.ctypes.data, None, 0) == 0
+
+
+@pytest.mark.parametrize("vocab", [256, 40000])
+@pytest.mark.parametrize("n_prompt", [1, 2, 5])
+def test_logits_that_are_all_nan(hiplib, vocab, n_prompt):
+    """The prompt's last token alone overflows behind the last layer's cache
+    writes: all its logits are NaN, its successor is -1, and generation goes on
+    as after token 0."""
+    announce(f"sample decode all NaN {vocab} {n_prompt}")
+    cfg = LlamaConfig(dim=64, hidden_dim=128, n_layers=1, n_heads=1, n_kv_heads=1, vocab_size=vocab, seq_len=64)
+    w, bad = scaled(cfg, 11), 77
+    # x[0] is 0 but for that token, whose feed-forward squares it, and x[1] takes
+    # the square times 1e40
+    w["tok_q"][:, 0] = 0
+    w["tok_q"][bad, 0] = 127
+    w["wo_q"][0, 0] = 0
+    w["w2_q"][0, 0] = 0
+    for name in ("w1", "w3"):
+        w[f"{name}_q"][0, 0] = 0
+        w[f"{name}_q"][0, 0, 0] = 127
+        w[f"{name}_s"][0, 0] = 1.0
+    w["w2_q"][0, 1] = 0
+    w["w2_q"][0, 1, 0] = 127
+    w["w2_s"][0, 1] = 3e38
+    w["w2_q"][0, 2:, 0] = 0
+    steps = 12
+    prompt = np.concatenate([make_prompt(cfg, n=n_prompt - 1, seed=2) % 70, [bad]]).astype(np.int32)
+    u = np.random.default_rng(n_prompt).random(steps, dtype=np.float32) * np.float32(0.9)
+    model = LlamaI8(hiplib, cfg, w)
+    try:
+        for how in (dict(temperature=0.8), dict(top_k=9), dict(top_p=0.9, min_p=0.01), dict(temperature=0.0)):
+            tokens, logprob = model.sample(prompt, u, **how)
+            eager = model.sample(prompt, u, graph=False, **how)
+            assert np.array_equal(tokens, eager[0]) and np.array_equal(logprob, eager[1]), how
+            assert tokens[0] == -1 and logprob[0] == -np.inf, how
+            text = np.concatenate([prompt, [0], tokens[1:-1]])
+            logits = model.logits(text)
+            where = np.isnan(logits)
+            assert where[n_prompt - 1].all() and not where[text != bad].any()
+            rows = [a if a is None else np.full(steps - 1, a) for a in
+                    (how.get("temperature"), how.get("top_k"), how.get("top_p"), how.get("min_p"))]
+            ok = np.zeros(steps - 1, bool)
+            for d in (-2e-4, 0.0, 2e-4):  # as above
+                want = ref.sample(logits[n_prompt:], *rows, np.clip(u[1:] + d, 0, 1))[0]
+                # a token after an overflowing one is again -1
+                ok |= np.where(text[n_prompt:] == bad, -1, want) == tokens[1:]
+            assert ok.all(), (how, tokens)
+    finally:
+        model.close()
