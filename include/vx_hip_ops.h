@@ -148,7 +148,10 @@ int32_t vx_nn_rope_append_f32(const float *qkv, const float *rope,
  * (what the others hold is never looked at); o: like q; lse: [batch, heads,
  * seq_q] f32 (may be NULL). With `causal`, query i of sequence b sees key j
  * of shared ++ own iff j <= shared_len + lens[b] - seq_q + i; else all
- * shared_len + lens[b]. A key that a query does not see does not reach its
+ * shared_len + lens[b]. The softmax weights are rounded to bf16 for their product
+ * with v, as in vx_nn_flash_attention_fwd_bf16; scores, maxima and sums are f32 (o
+ * is off by 2.3e-3 of its size in the root mean square, where the rounding of o
+ * itself makes 1.7e-3). A key that a query does not see does not reach its
  * result, whatever its values; a query that sees none gets o = 0 and lse =
  * -inf. k_shared and v_shared may be NULL where shared_len is 0, k and v
  * where capacity is 0. head_dim 64 or 128; pointers 16-byte aligned; scale and

@@ -41,7 +41,10 @@ constexpr int64_t part_floats(int64_t rows, int head_dim) {
  * us besides its blocks, and its partial results as much traffic as 130 keys:
  * 64 sequences of 32 heads on 4 over 8192 keys (16 tiles) 30 us in 16 splits,
  * 39 in 8 or 32; 128 sequences, 32 heads on 8, over 2048 31 in 4, 38 in 8; 16
- * over 4096 (8 tiles) 15 in 16, 19 in 8. */
+ * over 4096 (8 tiles) 15 in 16, 19 in 8. 64 at most, and 256 instead, for one tile:
+ * 4 sequences of 4 queries, 8 heads on 1, over 32768, 50000 and 131072 keys 23, 28
+ * and 50 us, and 26, 29 and 38; 4 of single queries 21, 26 and 47, and 20, 23 and
+ * 32; 2 of them, 4 heads on 1 (16 rows), 16.6, 19.5 and 30, and 17.8, 19.3 and 31. */
 inline int shared_splits(int64_t items, int64_t blocks, int cus) {
   int64_t s = std::min(cus / items, blocks / 8);
   if (items * s < cus / 2) {

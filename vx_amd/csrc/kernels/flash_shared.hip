@@ -30,12 +30,13 @@
  * another goes a key at a time where V there holds infinities or NaNs (0 x inf
  * is NaN), each key for the queries that see it.
  *
- * 16 sequences, 32 heads on 8 of 128, over 65536 shared and 128 own keys: 58 us
- * for 298 MB of keys, 5.1 TB/s, and 5 for the merge: the keys' bytes bound it. 64
- * on 4 KV heads over 8192: 25 and 5.3, where 10 would read the keys and 7 multiply;
- * a workgroup of 128 rows spends 8 us of its 25 before its first and after its
- * last block of 64 keys, and 1.7 on each. 8 sequences of 256 queries, 32 heads on
- * 8, over 4096 and 300 own, causal: 176 us, 810 TFLOP/s.
+ * 16 sequences, 32 heads on 8 of 128, over 65536 shared keys and own caches of up
+ * to 1024 (7176 keys in all): 58 us for 298 MB of keys, 5.1 TB/s, and 5 for the
+ * merge: the keys' bytes bound it. 64 on 4 KV heads over 8192: 25 and 5.3, where 10
+ * would read the keys and 7 multiply; a workgroup of 128 rows, one wave a SIMD,
+ * spends 8 us of its 25 before its first and after its last block of 64 keys, and
+ * 1.7 on each. 8 sequences of 256 queries, 32 heads on 8, over 4096 and 300 own,
+ * causal: 172 to 187 us by box, 830 to 760 TFLOP/s.
  */
 #include "../vx_batch_kernels.h"
 #include "../vx_hip_common.h"

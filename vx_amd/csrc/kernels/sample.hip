@@ -26,13 +26,16 @@
  * slice that the draw falls in, or the last to leave its few tokens, does the
  * rest.
  *
- * Latency bounds the small calls. 1 x 32000 f32 by top-k and top-p 10.1 us: 4.1
- * for the row's 128 KB into LDS by one workgroup, 1.5 for the maxima and their
- * bin, 3.1 for the list, 3.3 for the rest; 48 x 32000 with every setting in use
- * 22.8, of which the 64-bit weights of rows with top-p alone, 32 a thread, take
- * 11 (atomics for the tokens near the border alone save nothing). 8 x 131072 by top-p 23.5 in three launches (3.1, 7.4,
- * 13.0). 256 x 131071 without a border 64: the row out of memory twice, 269 MB at
- * 4.2 TB/s, and 512 64-bit weights a thread, 33 us on one CU.
+ * Latency bounds the small calls. 1 x 32000 f32 by top-k 11.6 us (10.2 at best),
+ * of which 2.7 for the row's 128 KB into LDS and its largest logit by one
+ * workgroup, 1.4 for the threads' maxima and their bin, 3.1 for the list and 3.1
+ * for the rest; 48 x 32000 with every setting in use 23, of which the 64-bit
+ * weights of rows with top-p alone, 32 a thread, take 11 (atomics for the tokens
+ * near the border alone save nothing). 8 x 131072 by top-p 30 a call, its three
+ * launches 4.5, 8.8 and 14 (3.9, 8.2 and 12.6 at best). 256 x 131071 without a
+ * border 64: the row out of memory twice and a sixteenth of it a third time, 276
+ * MB at 4.3 TB/s, and 128 64-bit weights a thread, 33 us on one CU; by top-p 160,
+ * the row three times and the histogram's weights.
  */
 #include "../vx_batch_kernels.h"
 #include "../vx_hip_common.h"
@@ -1225,7 +1228,10 @@ __device__ __forceinline__ void finish_slices(const SampleArgs &a, Shared &sh, i
 
 /* The rest: without a border the first slice finds the slice that the draw falls
  * in and its token; with one, the slices' tokens down to its bin (or, too many, of
- * that bin) meet in the workspace, and the last slice goes on with them. */
+ * that bin) meet in the workspace, and the last slice goes on with them. Where the
+ * tokens are too many and top_k or min_p is on, one workgroup goes over the whole
+ * row: 1 x 131072 f32 by top-k of 2000 123 us (133 undivided), by top-p 0.9999 with
+ * min-p 1e-5 at a temperature of 1.5 113 (146), by that top-p alone 35 (146). */
 template <bool kF32> __global__ __launch_bounds__(kThreads) void sample_settle(SampleArgs a, Split p) {
   __shared__ Shared sh;
   __shared__ u64 list[kBinList];
