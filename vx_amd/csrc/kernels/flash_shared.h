@@ -105,13 +105,10 @@ inline SharedPlan flash_shared_plan(int64_t batch, int heads, int kv_heads, int 
   const int64_t items = batch * kv_heads * p.own_tiles;
   if (may_split && p.own_splits) {
     /* up to one workgroup a CU, where it makes up for the merge (16 sequences
-     * of 32 heads on 8, 1024 own keys each: 65 us in 2 splits, 66 in 1, 68 in 4).
-     * One sequence over 33000 and 131072 keys, 8 heads on 1 of 128: 20 and 25 us
-     * so, 27 and 82 in 16 splits, 20 and 30 in 64; 32 heads on 8: 36 and 100, 42
-     * and 114 in 16; 30 queries of 8 heads on 2 over 33000: 31 and 63. */
+     * of 32 heads on 8, 1024 own keys each: 65 us in 2 splits, 66 in 1, 68 in 4) */
     const int64_t keys = p.together ? shared_len + (int64_t)capacity : capacity;
     p.own_splits = (int)std::max<int64_t>(
-        1, std::min<int64_t>(cus / items, keys / (p.together && p.own_rows ? 1024 : 512)));
+        1, std::min<int64_t>({cus / items, keys / (p.together && p.own_rows ? 1024 : 512), 16}));
   }
   p.own_groups = (int)(items * p.own_splits);
   p.parts = p.shared_splits + p.own_splits;
