@@ -416,6 +416,10 @@ def test_a_large_workspace_is_not_kept(hiplib):
 PLANNED = [
     ((1, 2, 1, 1, 1500, 700), [699], (1, 0, 1, 64, 0, 2)),
     ((1, 2, 2, 3, 9000, 300), [300], (1, 0, 1, 64, 0, 9)),
+    # no more than 16
+    ((1, 2, 1, 1, 33000, 300), [300], (1, 0, 1, 64, 0, 16)),
+    ((1, 4, 1, 8, 17000, 100), [77], (1, 0, 0, 64, 0, 16)),
+    ((1, 1, 1, 1, 0, 270000), [269999], (1, 0, 1, 64, 0, 16)),
     ((3, 8, 2, 5, 200, 60), [60, 5, 33], (1, 0, 0, 64, 0, 1)),
     ((1, 4, 1, 6, 3000, 1300), [1201], (1, 0, 0, 64, 0, 8)),
     ((1, 8, 1, 5, 5100, 70), [70], (1, 0, 0, 64, 0, 10)),

@@ -105,7 +105,13 @@ inline SharedPlan flash_shared_plan(int64_t batch, int heads, int kv_heads, int 
   const int64_t items = batch * kv_heads * p.own_tiles;
   if (may_split && p.own_splits) {
     /* up to one workgroup a CU, where it makes up for the merge (16 sequences
-     * of 32 heads on 8, 1024 own keys each: 65 us in 2 splits, 66 in 1, 68 in 4) */
+     * of 32 heads on 8, 1024 own keys each: 65 us in 2 splits, 66 in 1, 68 in 4),
+     * and 16: the lengths are not known here, and the parts of an emptier cache
+     * are merged for nothing. One sequence, 8 heads on 1 of 128, a cache of 131072
+     * with 500, 16000 and all keys in it: 8.7, 17 and 81 us in 16, 9.7, 14 and 46
+     * in 32, 11, 13.5 and 30 in 64, 15, 16 and 25 in 128; with 8 queries 11, 28 and
+     * 157, and in 64 14, 17 and 50; 32 heads on 8: 9.1, 19 and 109, and in 32 9.9,
+     * 19 and 97 */
     const int64_t keys = p.together ? shared_len + (int64_t)capacity : capacity;
     p.own_splits = (int)std::max<int64_t>(
         1, std::min<int64_t>({cus / items, keys / (p.together && p.own_rows ? 1024 : 512), 16}));
