@@ -36,7 +36,7 @@
  * would read the keys and 7 multiply; a workgroup of 128 rows, one wave a SIMD,
  * spends 8 us of its 25 before its first and after its last block of 64 keys, and
  * 1.7 on each. 8 sequences of 256 queries, 32 heads on 8, over 4096 and 300 own,
- * causal: 172 to 187 us by box, 830 to 760 TFLOP/s.
+ * causal: 172 to 187 us from one card to another, 830 to 760 TFLOP/s.
  */
 #include "../vx_batch_kernels.h"
 #include "../vx_hip_common.h"

@@ -1330,8 +1330,8 @@ template <bool kF32> void launch(const SampleArgs &a, const SamplePlan &plan, ch
 /* In us, several workgroups a row and one: 1 x 131072 f32 by top-k 22 and 25, by
  * top-p 23 and 69, without a border 20 and 48; 100 x 131072 without one 55 and
  * 59, 150 66 and 60, 256 92 and 73; 256 with one 190 and 226; 64 by top-k 38 and
- * 31, by top-p 60 and 122. At 50000 top-k 22 and 16, top-p 23 and 33. Up to 32768 one workgroup has the row in LDS (1 x
- * 32000 12 and 23). */
+ * 31, by top-p 60 and 122. At 50000 top-k 22 and 16, top-p 23 and 33. Up to 32768
+ * one workgroup has the row in LDS (1 x 32000 12 and 23). */
 SamplePlan sample_plan(int64_t rows, int64_t vocab, bool borders, bool may_split) {
   SamplePlan p{1, 0, 0};
   const int64_t chunks = (vocab + kChunk - 1) / kChunk;
