@@ -212,6 +212,121 @@ int32_t vx_nn_sample_bf16(const uint16_t *logits, const float *temperature,
  * extents it does not take. */
 int64_t vx_nn_sample_workspace(int64_t rows, int64_t vocab);
 
+/* ---- A packed batch in 8 bits --------------------------------------------
+ *
+ * Texts of different lengths in one run, their tokens one behind the other
+ * without padding, and activations in 8 bits against int8 weights: the norm (or
+ * plain quantization) that makes them, the product that reads them, attention
+ * that keeps the texts apart, and what the classifier's logits say of given
+ * tokens. vx_nn_rope_append_* turns a packed projection's heads as one sequence
+ * whose table has a row a token. No counterpart in the reference.
+ *
+ * Arguments, devices and `workspace` as for many answers to one prompt above
+ * (log probabilities use at most 160 KiB, the product 128 MiB). Outputs must not
+ * overlap inputs but where it is said. */
+
+/* The residual's addition and RMS norm of rows: s = x + residual, y = s *
+ * (mean s^2 + eps)^-1/2 * weight, the mean in 64 bits.
+ * x: [rows, dim], rows `stride` elements apart; residual: [rows, dim] (NULL: 0);
+ * weight: [dim] f32 (NULL: 1). Outputs, each of which may be NULL, one of y and
+ * q not: sum: [rows, dim], s rounded to x's type (the norm is of s itself); y:
+ * [rows, dim] bf16; q: [rows, dim] int8 with q_scale: [rows] f32, y in 8 bits: with
+ * t = s * weight in f32 and u = max |t| / 127 (1 where that is 0), q = t / u rounded
+ * to the nearest, half to even, and q_scale = u * (mean s^2 + eps)^-1/2.
+ * A row in which a t is not finite gets q = 0 and q_scale = NaN. sum may be x
+ * (where stride is dim) or residual itself. dim at most 32768, rows 2^21. */
+int32_t vx_nn_rms_norm_bf16(const uint16_t *x, const uint16_t *residual,
+                            const float *weight, uint16_t *sum, uint16_t *y,
+                            int8_t *q, float *q_scale, int64_t rows,
+                            int64_t dim, int64_t stride, float eps);
+int32_t vx_nn_rms_norm_f32(const float *x, const float *residual,
+                           const float *weight, float *sum, uint16_t *y,
+                           int8_t *q, float *q_scale, int64_t rows, int64_t dim,
+                           int64_t stride, float eps);
+
+/* Rows in 8 bits: q = x / u rounded to the nearest, half to even, q_scale = u =
+ * max |x| / 127 of the row (1 where that is 0). As above otherwise. */
+int32_t vx_nn_quantize_i8_bf16(const uint16_t *x, int8_t *q, float *q_scale,
+                               int64_t rows, int64_t dim, int64_t stride);
+int32_t vx_nn_quantize_i8_f32(const float *x, int8_t *q, float *q_scale,
+                              int64_t rows, int64_t dim, int64_t stride);
+
+/* int8 activations times int8 weights: y[t, r] = x_scale[t] * w_scale[r] *
+ * sum_c x[t, c] * w[r, c].
+ * x: [tokens, cols] int8; x_scale: [tokens] f32; w: [rows, cols] int8; w_scale:
+ * [rows] f32 (the weights of vx_nn_gemv_i8_bf16); y: [tokens, rows], rows
+ * `stride` elements apart (at least `rows`), bf16 or f32. The sum is exact; it
+ * is rounded to f32, multiplied by x_scale, then by w_scale, in f32, and rounded
+ * to y's type. cols a multiple of 16, at most 131056; x and w 16-byte aligned;
+ * tokens and rows at most 2^24. */
+int32_t vx_nn_gemm_i8_bf16(const int8_t *x, const float *x_scale,
+                           const int8_t *w, const float *w_scale, uint16_t *y,
+                           int64_t tokens, int64_t rows, int64_t cols,
+                           int64_t stride, void *workspace,
+                           int64_t workspace_bytes);
+int32_t vx_nn_gemm_i8_f32(const int8_t *x, const float *x_scale,
+                          const int8_t *w, const float *w_scale, float *y,
+                          int64_t tokens, int64_t rows, int64_t cols,
+                          int64_t stride, void *workspace,
+                          int64_t workspace_bytes);
+/* Bytes of workspace that such a call uses (0: none); a negative VX_OP_E* code
+ * for extents it does not take. */
+int64_t vx_nn_gemm_i8_workspace(int64_t tokens, int64_t rows, int64_t cols);
+
+/* Attention of packed sequences, each over its own keys.
+ * q, o: `total` rows of `heads` heads of head_dim bf16; k, v: the same of
+ * kv_heads heads. Row i of head h lies i * q_row + h * q_head elements from q
+ * (o_row and o_head from o, kv_row and kv_head from k and v alike): [heads,
+ * total, head_dim] as well as slices of a projection [total, heads + 2 *
+ * kv_heads, head_dim]. offsets (device memory, int32 [sequences + 1], read when
+ * the kernels run): sequence s has rows offsets[s] .. offsets[s + 1] - 1, none
+ * where those are equal. Rows before the first and from the last offset on
+ * belong to no sequence: they are not read, and their outputs stay as they
+ * were. offsets must not fall; where they do or lie outside 0 .. total, nothing
+ * outside the tensors is read or written, but which outputs are is not said.
+ * lse: [heads, total] f32 (may be NULL), natural logarithm.
+ * With `causal`, a query sees its sequence's keys up to its own row; else all.
+ * Numerics, `scale` and what hidden keys may hold as in
+ * vx_nn_flash_attention_shared_bf16. head_dim 64 or 128; strides multiples of 8,
+ * at least head_dim; kv_row at most 2^22; pointers 16-byte aligned; at most
+ * 65536 sequences and 2^28 queries of all heads. */
+int32_t vx_nn_flash_attention_packed_bf16(
+    const uint16_t *q, const uint16_t *k, const uint16_t *v,
+    const int32_t *offsets, uint16_t *o, float *lse, int64_t total,
+    int64_t sequences, int64_t heads, int64_t kv_heads, int64_t head_dim,
+    int64_t q_row, int64_t q_head, int64_t kv_row, int64_t kv_head,
+    int64_t o_row, int64_t o_head, float scale, int32_t causal);
+
+/* Log probabilities of given tokens, entropy, and the likeliest tokens of each
+ * row of logits, of p = softmax(logits), natural logarithms.
+ * logits: [rows, vocab] f32 or bf16, rows `stride` elements apart (at least
+ * vocab); given: [rows, n_given] int32, logprob: [rows, n_given] f32 (a token
+ * outside 0 .. vocab - 1 gets -inf); entropy: [rows] f32 (may be NULL), -sum p
+ * ln p; top_tokens: [rows, n_top] int32, the tokens of the n_top largest logits,
+ * falling, the lower index first among equals, and top_logprob: [rows, n_top]
+ * f32 (may be NULL).
+ * A NaN logit counts as -inf, and what is -inf is no alternative: where fewer
+ * are left, the rest are token -1 with logprob -inf. Where a logit is +inf,
+ * those alone have a probability, the same for each; the alternatives keep
+ * their order. A row without a logit above -inf has logprob -inf and entropy 0.
+ * n_top 0..64, n_given 0..2^20, rows at most 2^21, vocab at most 2^30. */
+int32_t vx_nn_token_logprobs_f32(const float *logits, const int32_t *given,
+                                 float *logprob, float *entropy,
+                                 int32_t *top_tokens, float *top_logprob,
+                                 int64_t rows, int64_t vocab, int64_t stride,
+                                 int64_t n_given, int64_t n_top,
+                                 void *workspace, int64_t workspace_bytes);
+int32_t vx_nn_token_logprobs_bf16(const uint16_t *logits, const int32_t *given,
+                                  float *logprob, float *entropy,
+                                  int32_t *top_tokens, float *top_logprob,
+                                  int64_t rows, int64_t vocab, int64_t stride,
+                                  int64_t n_given, int64_t n_top,
+                                  void *workspace, int64_t workspace_bytes);
+/* Bytes of workspace that such a call uses (0: none); VX_OP_EINVAL for extents
+ * it does not take. */
+int64_t vx_nn_token_logprobs_workspace(int64_t rows, int64_t vocab,
+                                       int64_t n_top);
+
 /* Greedy int8 decode of a Llama-2-style model, resident in HBM.
  *
  * The token step of reference examples/llama.vx:173-420 (RMSNorm eps 1e-5,

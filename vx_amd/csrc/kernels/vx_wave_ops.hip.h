@@ -1,11 +1,12 @@
 /*
- * vx_wave_ops.hip.h -- wave-wide reductions of the decoder's kernels
- * (decode.hip, prefill.hip), on VALU data movement.
+ * vx_wave_ops.hip.h -- wave-wide reductions on VALU data movement.
  */
 #ifndef VX_AMD_WAVE_OPS_HIP_H
 #define VX_AMD_WAVE_OPS_HIP_H
 
 #include <hip/hip_runtime.h>
+
+#include <cstdint>
 
 namespace vxk {
 namespace {
@@ -63,6 +64,32 @@ __device__ __forceinline__ float wave_max(float v) {
     v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
   }
   return v;
+}
+
+/* The word of the lane that reductions pair this one with at step kO: over
+ * steps 32, 16, 8, 4, 2, 1 in this order (or the reverse) each lane meets all
+ * others, and all end with the same bits where the operation commutes. */
+template <int kO> __device__ __forceinline__ uint32_t partner_word(uint32_t v) {
+  if constexpr (kO == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (threadIdx.x & 32) ? r[0] : r[1];
+  } else if constexpr (kO == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return (threadIdx.x & 16) ? r[0] : r[1];
+  } else {
+    constexpr int ctrl = kO == 8 ? 0x128 : kO == 4 ? 0x141 : kO == 2 ? 0x4e : 0xb1;
+    return __builtin_amdgcn_update_dpp(0u, v, ctrl, 0xf, 0xf, false);
+  }
+}
+
+__device__ __forceinline__ int wave_sum_int(int v) {
+  v += (int)partner_word<1>((uint32_t)v);
+  v += (int)partner_word<2>((uint32_t)v);
+  v += (int)partner_word<4>((uint32_t)v);
+  v += (int)partner_word<8>((uint32_t)v);
+  v += (int)partner_word<16>((uint32_t)v);
+  v += (int)partner_word<32>((uint32_t)v);
+  return __builtin_amdgcn_readfirstlane(v);
 }
 
 } // namespace

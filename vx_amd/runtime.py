@@ -72,6 +72,18 @@ HIP_SIGNATURES = {
     "vx_nn_sample_f32": (_i32, [_vp] * 8 + [_i64] * 3 + [_vp, _i64]),
     "vx_nn_sample_bf16": (_i32, [_vp] * 8 + [_i64] * 3 + [_vp, _i64]),
     "vx_nn_sample_workspace": (_i64, [_i64, _i64]),
+    "vx_nn_rms_norm_bf16": (_i32, [_vp] * 7 + [_i64] * 3 + [ctypes.c_float]),
+    "vx_nn_rms_norm_f32": (_i32, [_vp] * 7 + [_i64] * 3 + [ctypes.c_float]),
+    "vx_nn_quantize_i8_bf16": (_i32, [_vp] * 3 + [_i64] * 3),
+    "vx_nn_quantize_i8_f32": (_i32, [_vp] * 3 + [_i64] * 3),
+    "vx_nn_gemm_i8_bf16": (_i32, [_vp] * 5 + [_i64] * 4 + [_vp, _i64]),
+    "vx_nn_gemm_i8_f32": (_i32, [_vp] * 5 + [_i64] * 4 + [_vp, _i64]),
+    "vx_nn_gemm_i8_workspace": (_i64, [_i64] * 3),
+    "vx_nn_flash_attention_packed_bf16": (
+        _i32, [_vp] * 6 + [_i64] * 11 + [ctypes.c_float, _i32]),
+    "vx_nn_token_logprobs_f32": (_i32, [_vp] * 6 + [_i64] * 5 + [_vp, _i64]),
+    "vx_nn_token_logprobs_bf16": (_i32, [_vp] * 6 + [_i64] * 5 + [_vp, _i64]),
+    "vx_nn_token_logprobs_workspace": (_i64, [_i64] * 3),
     "vx_llama_i8_create": (_vp, [_vp, _vp, _u32]),
     "vx_llama_i8_generate": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _i32]),
     "vx_llama_i8_sample": (_i32, [_vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _i32]),
@@ -306,6 +318,57 @@ def sample(lib: DispatchLibrary, dtype: str, logits: int, temperature: int | Non
     fn = {"f32": lib.lib.vx_nn_sample_f32, "bf16": lib.lib.vx_nn_sample_bf16}[dtype]
     return fn(logits, temperature, top_k, top_p, min_p, u, tokens, logprob, rows, vocab,
               vocab if stride is None else stride, workspace, workspace_bytes)
+
+
+def rms_norm(lib: DispatchLibrary, dtype: str, x: int, residual: int | None, weight: int | None,
+             sum: int | None, y: int | None, q: int | None, q_scale: int | None, rows: int,
+             dim: int, eps: float, stride: int | None = None) -> int:
+    """vx_nn_rms_norm_<dtype> ("bf16" or "f32": the stream's type); stride None: dim."""
+    fn = lib.lib.vx_nn_rms_norm_bf16 if dtype == "bf16" else lib.lib.vx_nn_rms_norm_f32
+    return fn(x, residual, weight, sum, y, q, q_scale, rows, dim, dim if stride is None else stride,
+              eps)
+
+
+def quantize_i8(lib: DispatchLibrary, dtype: str, x: int, q: int, q_scale: int, rows: int, dim: int,
+                stride: int | None = None) -> int:
+    """vx_nn_quantize_i8_<dtype> ("bf16" or "f32": the rows' type); stride None: dim."""
+    fn = lib.lib.vx_nn_quantize_i8_bf16 if dtype == "bf16" else lib.lib.vx_nn_quantize_i8_f32
+    return fn(x, q, q_scale, rows, dim, dim if stride is None else stride)
+
+
+def gemm_i8(lib: DispatchLibrary, dtype: str, x: int, x_scale: int, w: int, w_scale: int, y: int,
+            tokens: int, rows: int, cols: int, stride: int | None = None,
+            workspace: int | None = None, workspace_bytes: int = 0) -> int:
+    """vx_nn_gemm_i8_<dtype> ("bf16" or "f32": the result's type); stride None: rows."""
+    fn = lib.lib.vx_nn_gemm_i8_bf16 if dtype == "bf16" else lib.lib.vx_nn_gemm_i8_f32
+    return fn(x, x_scale, w, w_scale, y, tokens, rows, cols, rows if stride is None else stride,
+              workspace, workspace_bytes)
+
+
+def flash_attention_packed(lib: DispatchLibrary, q: int, k: int, v: int, offsets: int, o: int,
+                           lse: int | None, total: int, sequences: int, heads: int, kv_heads: int,
+                           head_dim: int, scale: float, causal: bool,
+                           q_strides: tuple[int, int] | None = None,
+                           kv_strides: tuple[int, int] | None = None,
+                           o_strides: tuple[int, int] | None = None) -> int:
+    """vx_nn_flash_attention_packed_bf16; strides (row, head) in elements, None:
+    [heads, total, head_dim]."""
+    dense = (head_dim, total * head_dim)
+    return lib.lib.vx_nn_flash_attention_packed_bf16(
+        q, k, v, offsets, o, lse, total, sequences, heads, kv_heads, head_dim,
+        *(q_strides or dense), *(kv_strides or dense), *(o_strides or dense), scale,
+        1 if causal else 0)
+
+
+def token_logprobs(lib: DispatchLibrary, dtype: str, logits: int, given: int | None,
+                   logprob: int | None, entropy: int | None, top_tokens: int | None,
+                   top_logprob: int | None, rows: int, vocab: int, n_given: int, n_top: int,
+                   stride: int | None = None, workspace: int | None = None,
+                   workspace_bytes: int = 0) -> int:
+    """vx_nn_token_logprobs_<dtype> ("f32" or "bf16": the logits' type); stride None: vocab."""
+    fn = lib.lib.vx_nn_token_logprobs_bf16 if dtype == "bf16" else lib.lib.vx_nn_token_logprobs_f32
+    return fn(logits, given, logprob, entropy, top_tokens, top_logprob, rows, vocab,
+              vocab if stride is None else stride, n_given, n_top, workspace, workspace_bytes)
 
 
 class HipTimer:
