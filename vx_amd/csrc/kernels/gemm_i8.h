@@ -1,6 +1,6 @@
 /*
- * gemm_i8.h -- how an int8 product (gemm_i8.hip) is divided. Plain host
- * arithmetic.
+ * gemm_i8.h -- the choice of kernel, tile and splits of an int8 product
+ * (gemm_i8.hip). Plain host arithmetic.
  */
 #ifndef VX_AMD_GEMM_I8_H
 #define VX_AMD_GEMM_I8_H
@@ -14,27 +14,88 @@ namespace vxk {
 constexpr int64_t kGemmI8MaxCols = 131056;
 
 struct GemmI8Plan {
-  enum Kind { kFew, kTiles } kind;
-  int waves; /* kFew: waves that divide the columns of 16 rows */
+  enum Kind { kRow, kFew, kTiles } kind;
+  int tile;   /* kTiles: of i8::kTile */
   int splits; /* kTiles: workgroups that divide a tile's columns */
   int64_t ws_bytes;
 };
 
+namespace i8 {
+
+constexpr int kLine = 128; /* columns of a stage: a cache line of each row */
+
+/* Tiles of bm tokens x bn rows, and what one costs on a 256-CU MI355X: `fixed` us
+ * to start and store, and `stage` us a stage where every CU has per_cu of them,
+ * `alone` where it has one. At 32 stages (4096 columns), one tile a CU: 64x64 12.5
+ * us, 128x128 22, 128x192 29, 256x128 34, 256x256 57; two of 64x64 19.8. */
+struct Tile {
+  int bm, bn, per_cu;
+  double fixed, stage, alone;
+};
+constexpr Tile kTile[] = {{64, 64, 2, 1.7, 0.50, 0.27},
+                          {128, 128, 1, 3.2, 0.54, 0.54},
+                          {128, 192, 1, 4.8, 0.72, 0.72},
+                          {256, 128, 1, 5.5, 0.86, 0.86},
+                          {256, 256, 1, 9.5, 1.50, 1.50}};
+constexpr int kTiles = sizeof(kTile) / sizeof(kTile[0]);
+constexpr int kSplitTiles = 2; /* the first of them, which may be split */
+constexpr int kMaxSplits = 16;
+constexpr int64_t kMaxBytes = (int64_t)128 << 20;
+
+inline int64_t count(const Tile &t, int64_t tokens, int64_t rows) {
+  return ((tokens + t.bm - 1) / t.bm) * ((rows + t.bn - 1) / t.bn);
+}
+
+/* Splits leave 4 bytes a sum in a workspace, which a second launch reads. */
+inline int64_t ws_bytes(const Tile &t, int64_t tokens, int64_t rows, int splits) {
+  return splits > 1 ? count(t, tokens, rows) * splits * t.bm * t.bn * 4 : 0;
+}
+
+inline double us(const Tile &t, int64_t tokens, int64_t rows, int64_t cols, int splits, int cus) {
+  const int64_t units = count(t, tokens, rows) * splits, slots = (int64_t)t.per_cu * cus;
+  const int64_t full = units / slots, rest = units % slots;
+  const int64_t stages = ((cols + kLine - 1) / kLine + splits - 1) / splits;
+  double v = 2.5 + (double)full * (t.fixed + t.stage * (double)stages);
+  if (rest > 0) {
+    v += t.fixed + (rest <= cus ? t.alone : t.stage) * (double)stages;
+  }
+  return splits > 1 ? v + 3.0 + (double)ws_bytes(t, tokens, rows, splits) / 2e6 : v;
+}
+
+} // namespace i8
+
 inline GemmI8Plan gemm_i8_plan(int64_t tokens, int64_t rows, int64_t cols, int cus,
                                bool may_split) {
-  (void)may_split;
-  GemmI8Plan p{};
-  p.splits = 1;
-  if (tokens <= 64) {
-    p.kind = GemmI8Plan::kFew;
-    const int64_t groups = (rows + 15) / 16, stages = (cols + 63) / 64;
-    p.waves = 4;
-    while (p.waves < 16 && groups * p.waves < 8 * (int64_t)cus && stages > p.waves) {
-      p.waves *= 2;
-    }
-  } else {
-    p.kind = GemmI8Plan::kTiles;
+  GemmI8Plan p{GemmI8Plan::kTiles, 0, 1, 0};
+  if (tokens == 1) {
+    /* 32000 x 768 6.2 us, and 6.7 as few; 11008 x 4096 8.9 and 11.3 */
+    p.kind = GemmI8Plan::kRow;
+    return p;
   }
+  if (tokens <= 16 || (tokens <= 32 && rows * cols <= (int64_t(1) << 24))) {
+    /* 24 x 4096 x 4096 8.0 us, and 11 by tiles; 32 x 11008 x 4096 21 and 14, 32 x
+     * 32000 x 768 12.8 and 8.2; 16 x 11008 x 4096 14 and 13.3 */
+    p.kind = GemmI8Plan::kFew;
+    return p;
+  }
+  double best = 1e30;
+  for (int i = 0; i < i8::kTiles; ++i) {
+    const i8::Tile &t = i8::kTile[i];
+    const int64_t units = i8::count(t, tokens, rows), lines = (cols + i8::kLine - 1) / i8::kLine;
+    for (int s = 1; s <= (may_split && i < i8::kSplitTiles ? i8::kMaxSplits : 1); ++s) {
+      if (s > 1 && (units * s > (int64_t)t.per_cu * cus || lines < 4 * s ||
+                    i8::ws_bytes(t, tokens, rows, s) > i8::kMaxBytes)) {
+        break;
+      }
+      const double v = i8::us(t, tokens, rows, cols, s, cus);
+      if (v < best) {
+        best = v;
+        p.tile = i;
+        p.splits = s;
+      }
+    }
+  }
+  p.ws_bytes = i8::ws_bytes(i8::kTile[p.tile], tokens, rows, p.splits);
   return p;
 }
 

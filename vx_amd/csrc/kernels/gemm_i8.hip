@@ -12,6 +12,7 @@
 #include "../vx_packed_kernels.h"
 #include "gemm_pp_layout.h"
 #include "vx_lds_dma.hip.h"
+#include "vx_wave_ops.hip.h"
 
 #include <type_traits>
 
@@ -23,8 +24,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-
-constexpr int kStage = 64; /* columns of an MFMA */
 
 __device__ __forceinline__ i32x4 mfma_i8(u32x4 a, u32x4 b, i32x4 c) {
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a),
@@ -89,13 +88,92 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t rs, uint32_t off)
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, (int)off, 0, 0));
 }
 
-/* Up to 64 tokens: a workgroup has 16 rows of w and all tokens, its waves take
- * the stages in turn, each from memory into registers, and meet in LDS. */
-constexpr uint32_t kPast = 0x7ffffff0u; /* an offset past any buffer's end: reads zeros */
+/* One token: a wave has 4 rows of w, whose bytes it reads 1 KiB at a time of
+ * each, and adds up the products of its columns on v_dot4. With kSplit the four
+ * waves of a workgroup have the same rows and take the pieces in turn. */
+constexpr int kRowsEach = 4;
 
-template <bool kF32, int kTT, int kWaves>
+template <bool kF32, bool kSplit>
+__global__ __launch_bounds__(256) void gemm_i8_row(GemmI8Args a) {
+  constexpr int kPiece = 1024;
+  constexpr int kAhead = 2; /* pieces whose loads are in flight together */
+  __shared__ int part[kSplit ? 4 : 1][kRowsEach];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t r0 = ((int64_t)blockIdx.x * (kSplit ? 1 : 4) + (kSplit ? 0 : wave)) * kRowsEach;
+  if (r0 >= a.rows) {
+    return; /* (not with kSplit) */
+  }
+  const int cols = a.cols;
+  const int rows_here = (int)min((int64_t)kRowsEach, a.rows - r0);
+  int acc[kRowsEach] = {};
+  constexpr int kStep = kSplit ? 4 : 1;
+  const int pieces = (cols + kPiece - 1) / kPiece;
+  for (int p0 = kSplit ? wave : 0; p0 < pieces; p0 += kStep * kAhead) {
+    u32x4 w[kAhead][kRowsEach], x[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int c = (p0 + i * kStep) * kPiece + 16 * lane;
+      const bool in = c < cols;
+#pragma unroll
+      for (int r = 0; r < kRowsEach; ++r) {
+        w[i][r] = u32x4{0, 0, 0, 0};
+        if (in) {
+          w[i][r] = __builtin_nontemporal_load(reinterpret_cast<const u32x4 *>(
+              a.w + (r0 + min(r, rows_here - 1)) * cols + c));
+        }
+      }
+      x[i] = u32x4{0, 0, 0, 0};
+      if (in) {
+        x[i] = *reinterpret_cast<const u32x4 *>(a.x + c);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0); /* all loads before the first product */
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+#pragma unroll
+      for (int r = 0; r < kRowsEach; ++r) {
+        for (int e = 0; e < 4; ++e) {
+          acc[r] = __builtin_amdgcn_sdot4((int)w[i][r][e], (int)x[i][e], acc[r], false);
+        }
+      }
+    }
+  }
+  /* lane r stores row r's output */
+  int mine = 0;
+#pragma unroll
+  for (int r = 0; r < kRowsEach; ++r) {
+    const int sum = wave_sum_int(acc[r]);
+    mine = lane == r ? sum : mine;
+  }
+  if constexpr (kSplit) {
+    if (lane < kRowsEach) {
+      part[wave][lane] = mine;
+    }
+    __syncthreads();
+    if (wave != 0 || lane >= kRowsEach) {
+      return;
+    }
+    mine = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+  }
+  if (lane < rows_here) {
+    const float v = (float)mine * a.x_scale[0] * a.w_scale[r0 + lane];
+    if constexpr (kF32) {
+      static_cast<float *>(a.y)[r0 + lane] = v;
+    } else {
+      static_cast<uint16_t *>(a.y)[r0 + lane] = f32_to_bf16(v);
+    }
+  }
+}
+
+/* Few tokens: a workgroup has 16 rows of w and all tokens, its waves take lines
+ * of 128 columns in turn, kAhead at once, from memory into registers, and meet in
+ * LDS. */
+constexpr uint32_t kPast = 0x7ffffff0u; /* an offset past any buffer's end: reads zeros */
+using i8::kLine;
+
+template <bool kF32, int kTT, int kWaves, int kAhead>
 __global__ __launch_bounds__(64 * kWaves) void gemm_i8_few(GemmI8Args a) {
-  constexpr int kAhead = 4; /* stages whose loads are in flight together */
   __shared__ i32x4 part[kWaves][kTT][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -112,24 +190,31 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_i8_few(GemmI8Args a) {
   for (int i = 0; i < kTT; ++i) {
     acc[i] = i32x4{0, 0, 0, 0};
   }
-  const int stages = (cols + kStage - 1) / kStage;
-  for (int s0 = wave; s0 < stages; s0 += kWaves * kAhead) {
-    u32x4 wv[kAhead], xv[kAhead][kTT];
+  const int lines = (cols + kLine - 1) / kLine;
+  for (int s0 = wave; s0 < lines; s0 += kWaves * kAhead) {
+    u32x4 wv[kAhead][2], xv[kAhead][2][kTT];
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
-      const int c = (s0 + i * kWaves) * kStage + 16 * g;
-      const bool in = c < cols;
-      wv[i] = load16(wr, in ? (uint32_t)(l16 * cols + c) : kPast);
 #pragma unroll
-      for (int j = 0; j < kTT; ++j) {
-        xv[i][j] = load16(xr, in ? (uint32_t)((16 * j + l16) * cols + c) : kPast);
+      for (int h = 0; h < 2; ++h) {
+        const int c = (s0 + i * kWaves) * kLine + 64 * h + 16 * g;
+        const bool in = c < cols;
+        wv[i][h] = load16(wr, in ? (uint32_t)(l16 * cols + c) : kPast);
+#pragma unroll
+        for (int j = 0; j < kTT; ++j) {
+          xv[i][h][j] = load16(xr, in ? (uint32_t)((16 * j + l16) * cols + c) : kPast);
+        }
       }
     }
+    __builtin_amdgcn_sched_barrier(0); /* all loads before the first product */
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
 #pragma unroll
-      for (int j = 0; j < kTT; ++j) {
-        acc[j] = mfma_i8(wv[i], xv[i][j], acc[j]);
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int j = 0; j < kTT; ++j) {
+          acc[j] = mfma_i8(wv[i][h], xv[i][h][j], acc[j]);
+        }
       }
     }
   }
@@ -152,80 +237,78 @@ __global__ __launch_bounds__(64 * kWaves) void gemm_i8_few(GemmI8Args a) {
   }
 }
 
-/* Tiles of 128 tokens x 128 rows: four waves of 64x64, two workgroups to a CU,
- * stages of 64 columns through an LDS ring of five slots filled by
- * buffer-to-LDS loads. Planes are [128 rows][4 chunks of 16 columns], a chunk's
- * place XORed with the row's bits as in the 16-bit kernels. */
-constexpr int kBM = 128, kBN = 128, kTM = 4, kTN = 4, kNS = 5;
-constexpr int kUnitsA = kBM * 4, kUnitsB = kBN * 4;
-
-template <bool kF32>
-__global__ __launch_bounds__(256, 2) void gemm_i8_tiles(GemmI8Args a, int tiles_m, int tiles_n) {
-  constexpr int kLA = kUnitsA / 256, kLB = kUnitsB / 256;
+/* Tiles of kBM tokens x kBN rows on kWM x kWN waves: stages of 128 columns (a
+ * whole cache line of each row) through an LDS ring of kNS slots filled by
+ * buffer-to-LDS loads. Planes are [rows][8 chunks of 16 columns], chunk c of a row
+ * at place c ^ (row % 8), so that reads of 16 rows at one chunk meet every bank.
+ * With kMid a slot's plane of w is filled again from the middle of its stage on,
+ * when all of it is in registers. */
+template <bool kF32, int kBM, int kBN, int kWM, int kWN, int kNS, bool kMid, int kPerCu>
+__global__ __launch_bounds__(64 * kWM * kWN, kPerCu * kWM * kWN / 4) void gemm_i8_tiles(
+    GemmI8Args a, int tiles_m, int tiles_n, int splits, i32x4 *__restrict__ parts) {
+  constexpr int kThreads = 64 * kWM * kWN;
+  constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16; /* 16x16 blocks of a wave */
+  constexpr int kUnitsA = kBM * 8, kUnitsB = kBN * 8;       /* 16-byte units per stage */
+  constexpr int kLA = kUnitsA / kThreads, kLB = kUnitsB / kThreads;
+  constexpr int kLead = 2;        /* steps that A's reads run ahead */
+  constexpr int kSteps = 2 * kTM; /* of kTN products, a stage's */
+  static_assert(kUnitsA % kThreads == 0 && kUnitsB % kThreads == 0 && kLead <= kTM, "whole loads");
   __shared__ u32x4 ring[kNS][kUnitsA + kUnitsB];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int l16 = lane & 15;
   const int g = lane >> 4;
-  const int wm = wave >> 1, wn = wave & 1;
-  const pp::Tile tile = pp::tile_of(blockIdx.x, gridDim.x, tiles_m, tiles_n);
+  const int wm = wave / kWN, wn = wave % kWN;
+  const int tiles = tiles_m * tiles_n;
+  const int split = (int)blockIdx.x / tiles;
+  const int id = (int)blockIdx.x - split * tiles;
+  const pp::Tile tile = pp::tile_of(id, tiles, tiles_m, tiles_n);
   const int64_t m0 = (int64_t)tile.tm * kBM;
   const int64_t n0 = (int64_t)tile.tn * kBN;
+  /* this workgroup's stages */
+  const int all = (a.cols + kLine - 1) / kLine;
+  const int first = (int)((int64_t)all * split / splits);
+  const int stages = (int)((int64_t)all * (split + 1) / splits) - first;
   const int cols = a.cols;
-  const int stages = (cols + kStage - 1) / kStage;
-  const bool ragged = cols % kStage != 0;
 
-  /* Rows past the end read zeros; columns past the end of a row belong to the
-   * next one, and are left out on x's side. */
-  uint32_t a_off[kLA], b_off[kLB];
-  bool a_in[kLA]; /* in the last stage */
-#pragma unroll
-  for (int p = 0; p < kLA; ++p) {
-    const int u = (wave * kLA + p) * 64 + lane;
-    const int row = u >> 2, c = pp::dswz_a(row, u & 3) * 16;
-    a_off[p] = (uint32_t)(row * cols + c);
-    a_in[p] = (stages - 1) * kStage + c < cols;
-  }
-#pragma unroll
-  for (int p = 0; p < kLB; ++p) {
-    const int u = (wave * kLB + p) * 64 + lane;
-    const int row = u >> 2;
-    b_off[p] = (uint32_t)(row * cols + pp::dswz_a(row, u & 3) * 16);
-  }
+  /* Load p of a wave fills rows (wave * kLA + p) * 8 + lane / 8 of a plane; its
+   * offset is that of p = 0 and 8 p rows. Rows past the end read zeros; columns
+   * past the end of a row belong to the next one, and are left out on x's side. */
+  const int at_chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+  const uint32_t a_off = (uint32_t)((wave * kLA * 8 + (lane >> 3)) * cols + at_chunk);
+  const uint32_t b_off = (uint32_t)((wave * kLB * 8 + (lane >> 3)) * cols + at_chunk);
+  const bool cut = (all - 1) * kLine + at_chunk >= cols; /* in the row's last stage */
   const int a_end = (int)min((int64_t)kBM, a.tokens - m0) * cols;
   const int b_end = (int)min((int64_t)kBN, a.rows - n0) * cols;
   const uint32_t ring_base = (uint32_t)(uintptr_t)(VX_LDS void *)&ring[0][0];
-  auto issue = [&](int st, int slot) {
-    const int c0 = st * kStage;
-    const i32x4 ra = buffer_rsrc(a.x + m0 * cols + c0, a_end - c0);
-    const i32x4 rb = buffer_rsrc(a.w + n0 * cols + c0, b_end - c0);
-    const uint32_t base = ring_base + (uint32_t)(slot * (kUnitsA + kUnitsB) * 16);
-    const bool cut = ragged && st == stages - 1;
+  auto issue_a = [&](int st, int slot) {
+    const int c0 = (first + st) * kLine;
+    const i32x4 rs = buffer_rsrc(a.x + m0 * cols + c0, a_end - c0);
+    const uint32_t to = ring_base + (uint32_t)(slot * (kUnitsA + kUnitsB) * 16 + wave * kLA * 1024);
+    const bool last = first + st == all - 1;
 #pragma unroll
     for (int p = 0; p < kLA; ++p) {
-      dma16(ra, cut && !a_in[p] ? kPast : a_off[p], base + (uint32_t)((wave * kLA + p) * 1024));
+      dma16(rs, cut && last ? kPast : a_off + (uint32_t)(8 * p * cols), to + (uint32_t)(p * 1024));
     }
+  };
+  auto issue_b = [&](int st, int slot) {
+    const int c0 = (first + st) * kLine;
+    const i32x4 rs = buffer_rsrc(a.w + n0 * cols + c0, b_end - c0);
+    const uint32_t to =
+        ring_base + (uint32_t)((slot * (kUnitsA + kUnitsB) + kUnitsA) * 16 + wave * kLB * 1024);
 #pragma unroll
     for (int p = 0; p < kLB; ++p) {
-      dma16(rb, b_off[p], base + (uint32_t)(kUnitsA * 16 + (wave * kLB + p) * 1024));
+      dma16(rs, b_off + (uint32_t)(8 * p * cols), to + (uint32_t)(p * 1024));
     }
   };
 
-  struct Frags {
-    u32x4 a[kTM], b[kTN];
+  /* Blocks are 16 rows apart, so that their chunks' places are the same. */
+  const int at0 = l16 * 8 + (g ^ (l16 & 7)), at1 = l16 * 8 + ((4 + g) ^ (l16 & 7));
+  auto read_a = [&](int slot, int ks, int i) {
+    return ring[slot][(wm * kTM + i) * 128 + (ks ? at1 : at0)];
   };
-  auto read = [&](int slot, Frags &f) {
-    const u32x4 *la = ring[slot], *lb = la + kUnitsA;
-#pragma unroll
-    for (int j = 0; j < kTN; ++j) {
-      const int row = (wn * kTN + j) * 16 + l16;
-      f.b[j] = lb[row * 4 + pp::dswz_a(row, g)];
-    }
-#pragma unroll
-    for (int i = 0; i < kTM; ++i) {
-      const int row = (wm * kTM + i) * 16 + l16;
-      f.a[i] = la[row * 4 + pp::dswz_a(row, g)];
-    }
+  auto read_b = [&](int slot, int ks, int j) {
+    return ring[slot][kUnitsA + (wn * kTN + j) * 128 + (ks ? at1 : at0)];
   };
   i32x4 acc[kTM][kTN];
 #pragma unroll
@@ -235,53 +318,104 @@ __global__ __launch_bounds__(256, 2) void gemm_i8_tiles(GemmI8Args a, int tiles_
       acc[i][j] = i32x4{0, 0, 0, 0};
     }
   }
-  auto multiply = [&](const Frags &f) {
-#pragma unroll
-    for (int j = 0; j < kTN; ++j) {
-#pragma unroll
-      for (int i0 = 0; i0 < kTM; ++i0) {
-        const int i = (j & 1) ? kTM - 1 - i0 : i0;
-        acc[i][j] = mfma_i8(f.b[j], f.a[i], acc[i][j]);
-      }
-    }
-  };
 
 #pragma unroll
   for (int s = 0; s < kNS; ++s) {
     if (s < stages) {
-      issue(s, s);
+      issue_a(s, s);
+      issue_b(s, s);
     }
   }
   wait_stages<kNS - 1, kLA + kLB>(min(stages, kNS) - 1);
   lds_barrier();
-  Frags f0, f1;
-  read(0, f0);
-  /* Entering stage s: its operands are in `f`, and every wave's reads of them
-   * end before the barrier, after which its slot takes stage s + kNS. The
-   * next stage's reads run beside this one's MFMAs. */
-  int slot = 0;
-  auto stage = [&](int s, const Frags &f, Frags &next) {
-    wait_stages<kNS - 2, kLA + kLB>(min(stages - 2 - s, kNS - 2));
-    lds_barrier();
-    if (s + kNS < stages) {
-      issue(s + kNS, slot);
-    }
-    slot = slot == kNS - 1 ? 0 : slot + 1;
-    read(slot, next);
-    multiply(f);
-  };
-  int s = 0;
-  for (; s + 2 < stages; s += 2) {
-    stage(s, f0, f1);
-    stage(s + 1, f1, f0);
+  u32x4 b0[kTN], b1[kTN], av[kLead];
+#pragma unroll
+  for (int j = 0; j < kTN; ++j) {
+    b0[j] = read_b(0, 0, j);
   }
-  if (s + 1 < stages) {
-    stage(s, f0, f1);
-    multiply(f1);
-  } else {
-    multiply(f0);
+#pragma unroll
+  for (int i = 0; i < kLead; ++i) {
+    av[i] = read_a(0, 0, i);
+  }
+  /* Entering stage s, its first B operands are in b0 and its first A operands in
+   * av. kLead steps before its end every wave has read all of it: the next stage's
+   * loads are waited for, and past the barrier its first operands are read and the
+   * slot takes stage s + kNS. (kMid: its plane of w was read by the middle.) */
+  int slot = 0;
+  for (int s = 0; s < stages; ++s) {
+    const int after = slot == kNS - 1 ? 0 : slot + 1;
+    const bool more = s + kNS < stages;
+#pragma unroll
+    for (int r = 0; r < kSteps; ++r) {
+      const int ks = r / kTM, i = r % kTM;
+      __builtin_amdgcn_sched_barrier(0);
+      if (kMid && r == kTM) {
+        lds_barrier();
+        if (more) {
+          issue_b(s + kNS, slot);
+        }
+      }
+      if (r == kSteps - kLead) {
+        if constexpr (kMid) {
+          /* newer than stage s + 1: whole stages, and the plane just issued */
+          if (more) {
+            wait_vm<(kNS - 2) * (kLA + kLB) + kLB>();
+          } else {
+            wait_stages<kNS - 2, kLA + kLB>(min(stages - 2 - s, kNS - 2));
+          }
+        } else {
+          wait_stages<kNS - 2, kLA + kLB>(min(stages - 2 - s, kNS - 2));
+        }
+        lds_barrier();
+        if (more) {
+          issue_a(s + kNS, slot);
+          if (!kMid) {
+            issue_b(s + kNS, slot);
+          }
+        }
+      }
+      const int n = r + kLead; /* the step that this one's read is for */
+      const u32x4 an = n < kSteps ? read_a(slot, n / kTM, n % kTM) : read_a(after, 0, n - kSteps);
+      if (ks == 0) {
+        constexpr int kPer = (kTN + kTM - 1) / kTM;
+#pragma unroll
+        for (int j = i * kPer; j < min((i + 1) * kPer, kTN); ++j) {
+          b1[j] = read_b(slot, 1, j);
+        }
+      } else if (r >= kSteps - kLead) {
+        /* in place of those that this step's products no longer need */
+        constexpr int kPer = (kTN + kLead - 1) / kLead;
+        const int e = r - (kSteps - kLead);
+#pragma unroll
+        for (int j = e * kPer; j < min((e + 1) * kPer, kTN); ++j) {
+          b0[j] = read_b(after, 0, j);
+        }
+      }
+#pragma unroll
+      for (int j0 = 0; j0 < kTN; ++j0) {
+        const int j = (i & 1) ? kTN - 1 - j0 : j0;
+        acc[i][j] = mfma_i8(ks ? b1[j] : b0[j], av[0], acc[i][j]);
+      }
+#pragma unroll
+      for (int e = 0; e + 1 < kLead; ++e) {
+        av[e] = av[e + 1];
+      }
+      av[kLead - 1] = an;
+    }
+    slot = after;
   }
 
+  if (splits > 1) {
+    i32x4 *to = parts + ((int64_t)blockIdx.x * kTM * kTN) * kThreads + threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kTM; ++i) {
+#pragma unroll
+      for (int j = 0; j < kTN; ++j) {
+        to[(i * kTN + j) * kThreads] = acc[i][j];
+      }
+    }
+    return;
+  }
   const bool aligned = aligned_rows<kF32>(a);
 #pragma unroll
   for (int j = 0; j < kTN; ++j) {
@@ -300,36 +434,99 @@ __global__ __launch_bounds__(256, 2) void gemm_i8_tiles(GemmI8Args a, int tiles_
   }
 }
 
-template <bool kF32, int kTT> void few(const GemmI8Args &a, int waves, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.rows + 15) / 16));
-  if (waves == 4) {
-    hipLaunchKernelGGL((gemm_i8_few<kF32, kTT, 4>), grid, dim3(256), 0, stream, a);
-  } else if (waves == 8) {
-    hipLaunchKernelGGL((gemm_i8_few<kF32, kTT, 8>), grid, dim3(512), 0, stream, a);
+/* The sums of a tile's splits, a thread a register of the kernel that left them. */
+template <bool kF32, int kBM, int kBN, int kWM, int kWN>
+__global__ __launch_bounds__(256) void gemm_i8_join(GemmI8Args a, int tiles_m, int tiles_n,
+                                                    int splits, const i32x4 *__restrict__ parts) {
+  constexpr int kThreads = 64 * kWM * kWN;
+  constexpr int kTM = kBM / kWM / 16, kTN = kBN / kWN / 16;
+  constexpr int kPart = kTM * kTN * kThreads; /* of a tile */
+  const int tiles = tiles_m * tiles_n;
+  const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int id = (int)(at / kPart), u = (int)(at % kPart);
+  if (id >= tiles) {
+    return;
+  }
+  const pp::Tile tile = pp::tile_of(id, tiles, tiles_m, tiles_n);
+  const int block = u / kThreads, thread = u % kThreads;
+  const int wave = thread >> 6, l16 = thread & 15, g = (thread & 63) >> 4;
+  const int64_t r = (int64_t)tile.tn * kBN + (wave % kWN * kTN + block % kTN) * 16 + 4 * g;
+  const int64_t t = (int64_t)tile.tm * kBM + (wave / kWN * kTM + block / kTN) * 16 + l16;
+  if (r >= a.rows || t >= a.tokens) {
+    return;
+  }
+  i32x4 sum = {0, 0, 0, 0};
+  for (int s = 0; s < splits; ++s) {
+    sum += parts[((int64_t)s * tiles + id) * kPart + u];
+  }
+  put4<kF32>(a, t, r, sum, a.x_scale[t], scales4(a.w_scale, r, a.rows),
+             aligned_rows<kF32>(a) && r + 4 <= a.rows);
+}
+
+template <bool kF32> void row(const GemmI8Args &a, hipStream_t stream) {
+  const unsigned groups = (unsigned)((a.rows + kRowsEach - 1) / kRowsEach);
+  /* 11008 x 4096 12.7 us undivided, 8.9 divided; 16384 x 2048 7.2 and 7.7 */
+  if (a.cols > 2048) {
+    hipLaunchKernelGGL((gemm_i8_row<kF32, true>), dim3(groups), dim3(256), 0, stream, a);
   } else {
-    hipLaunchKernelGGL((gemm_i8_few<kF32, kTT, 16>), grid, dim3(1024), 0, stream, a);
+    hipLaunchKernelGGL((gemm_i8_row<kF32, false>), dim3((groups + 3) / 4), dim3(256), 0, stream, a);
   }
 }
 
-template <bool kF32> void launch(const GemmI8Args &a, const GemmI8Plan &p, hipStream_t stream) {
-  if (p.kind == GemmI8Plan::kFew) {
-    if (a.tokens <= 16) {
-      few<kF32, 1>(a, p.waves, stream);
-    } else if (a.tokens <= 32) {
-      few<kF32, 2>(a, p.waves, stream);
-    } else {
-      few<kF32, 4>(a, p.waves, stream);
-    }
-    return;
+template <bool kF32, int kTT, int kWaves, int kAhead>
+void few_ahead(const GemmI8Args &a, hipStream_t stream) {
+  hipLaunchKernelGGL((gemm_i8_few<kF32, kTT, kWaves, kAhead>), dim3((unsigned)((a.rows + 15) / 16)),
+                     dim3(64 * kWaves), 0, stream, a);
+}
+template <bool kF32, int kTT> void few(const GemmI8Args &a, hipStream_t stream) {
+  const int lines = (a.cols + kLine - 1) / kLine;
+  if (lines <= 4) {
+    few_ahead<kF32, kTT, 4, 1>(a, stream);
+  } else if (lines <= 8) {
+    few_ahead<kF32, kTT, 8, 1>(a, stream);
+  } else if (kTT > 1 || lines <= 16) {
+    few_ahead<kF32, kTT, 8, 2>(a, stream);
+  } else {
+    few_ahead<kF32, kTT, 8, kTT == 1 ? 4 : 2>(a, stream);
   }
+}
+
+template <bool kF32, int kBM, int kBN, int kWM, int kWN, int kNS, bool kMid, int kPerCu>
+void tiles(const GemmI8Args &a, int splits, char *ws, hipStream_t stream) {
   const int tm = (int)((a.tokens + kBM - 1) / kBM), tn = (int)((a.rows + kBN - 1) / kBN);
-  hipLaunchKernelGGL((gemm_i8_tiles<kF32>), dim3((unsigned)(tm * tn)), dim3(256), 0, stream, a, tm, tn);
+  hipLaunchKernelGGL((gemm_i8_tiles<kF32, kBM, kBN, kWM, kWN, kNS, kMid, kPerCu>),
+                     dim3((unsigned)(tm * tn * splits)), dim3(64 * kWM * kWN), 0, stream, a, tm, tn,
+                     splits, reinterpret_cast<i32x4 *>(ws));
+  if (splits > 1) {
+    const int64_t all = (int64_t)tm * tn * (kBM * kBN / 4);
+    hipLaunchKernelGGL((gemm_i8_join<kF32, kBM, kBN, kWM, kWN>), dim3((unsigned)((all + 255) / 256)),
+                       dim3(256), 0, stream, a, tm, tn, splits, reinterpret_cast<const i32x4 *>(ws));
+  }
+}
+
+template <bool kF32>
+void launch(const GemmI8Args &a, const GemmI8Plan &p, char *ws, hipStream_t stream) {
+  if (p.kind == GemmI8Plan::kRow) {
+    row<kF32>(a, stream);
+  } else if (p.kind == GemmI8Plan::kFew) {
+    a.tokens <= 16 ? few<kF32, 1>(a, stream) : few<kF32, 2>(a, stream);
+  } else if (p.tile == 0) {
+    tiles<kF32, 64, 64, 2, 2, 4, false, 2>(a, p.splits, ws, stream);
+  } else if (p.tile == 1) {
+    tiles<kF32, 128, 128, 4, 2, 4, false, 1>(a, p.splits, ws, stream);
+  } else if (p.tile == 2) {
+    tiles<kF32, 128, 192, 4, 2, 3, false, 1>(a, 1, nullptr, stream);
+  } else if (p.tile == 3) {
+    tiles<kF32, 256, 128, 4, 2, 3, false, 1>(a, 1, nullptr, stream);
+  } else {
+    tiles<kF32, 256, 256, 4, 2, 2, true, 1>(a, 1, nullptr, stream);
+  }
 }
 
 } // namespace
 
-void gemm_i8_launch(const GemmI8Args &a, const GemmI8Plan &plan, char *, hipStream_t stream) {
-  a.f32 ? launch<true>(a, plan, stream) : launch<false>(a, plan, stream);
+void gemm_i8_launch(const GemmI8Args &a, const GemmI8Plan &plan, char *ws, hipStream_t stream) {
+  a.f32 ? launch<true>(a, plan, ws, stream) : launch<false>(a, plan, ws, stream);
 }
 
 } // namespace vxk
