@@ -24,19 +24,21 @@ namespace i8 {
 
 constexpr int kLine = 128; /* columns of a stage: a cache line of each row */
 
-/* Tiles of bm tokens x bn rows, and what one costs on a 256-CU MI355X: `fixed` us
- * to start and store, and `stage` us a stage where every CU has per_cu of them,
- * `alone` where it has one. At 32 stages (4096 columns), one tile a CU: 64x64 12.5
- * us, 128x128 22, 128x192 29, 256x128 34, 256x256 57; two of 64x64 19.8. */
+/* Tiles of bm tokens x bn rows, per_cu of them to a CU, and what a round of them
+ * takes on a 256-CU MI355X: `fixed` us to start and store, and a stage `full` us
+ * where all CUs have their per_cu, `some` where few have one (two to a CU: where
+ * all have one). At 32 stages (4096 columns), rounds of 256 and of fewer tiles:
+ * 64x64 13 us, and two to a CU 19.6; 128x128 24.5 (86: 20), 128x192 28.3 (176:
+ * 27.3), 256x128 36.6 (128: 32), 256x256 59 (96: 49), two of 128x128 37 (256:
+ * 28.5); at 2 stages 128x128 4.1, two of them 5.5, 128x192 5.2, 256x128 6.2, 256x256
+ * 12.4. Two of 128x128 have a ring of two slots each, one alone of four. */
 struct Tile {
   int bm, bn, per_cu;
-  double fixed, stage, alone;
+  double fixed, full, some;
 };
-constexpr Tile kTile[] = {{64, 64, 2, 1.7, 0.50, 0.27},
-                          {128, 128, 1, 3.2, 0.54, 0.54},
-                          {128, 192, 1, 4.8, 0.72, 0.72},
-                          {256, 128, 1, 5.5, 0.86, 0.86},
-                          {256, 256, 1, 9.5, 1.50, 1.50}};
+constexpr Tile kTile[] = {{64, 64, 2, 2.1, 0.42, 0.25},   {128, 128, 1, 2.9, 0.60, 0.42},
+                          {128, 128, 2, 3.4, 1.05, 0.70}, {128, 192, 1, 3.65, 0.78, 0.45},
+                          {256, 128, 1, 4.2, 0.98, 0.65}, {256, 256, 1, 7.4, 1.55, 1.00}};
 constexpr int kTiles = sizeof(kTile) / sizeof(kTile[0]);
 constexpr int kSplitTiles = 2; /* the first of them, which may be split */
 constexpr int kMaxSplits = 16;
@@ -55,9 +57,11 @@ inline double us(const Tile &t, int64_t tokens, int64_t rows, int64_t cols, int 
   const int64_t units = count(t, tokens, rows) * splits, slots = (int64_t)t.per_cu * cus;
   const int64_t full = units / slots, rest = units % slots;
   const int64_t stages = ((cols + kLine - 1) / kLine + splits - 1) / splits;
-  double v = 2.5 + (double)full * (t.fixed + t.stage * (double)stages);
+  double v = 2.5 + (double)full * (t.fixed + t.full * (double)stages);
   if (rest > 0) {
-    v += t.fixed + (rest <= cus ? t.alone : t.stage) * (double)stages;
+    const int64_t from = t.per_cu > 1 ? cus : 0; /* `some` up to here */
+    const double more = (double)std::max<int64_t>(rest - from, 0) / (double)(slots - from);
+    v += t.fixed + (t.some + (t.full - t.some) * more) * (double)stages;
   }
   return splits > 1 ? v + 3.0 + (double)ws_bytes(t, tokens, rows, splits) / 2e6 : v;
 }
