@@ -20,9 +20,20 @@
  * product's operands are bf16 (f32 ones multiply at a sixteenth of the rate);
  * maxima and sums stay in f32, the sums over unrounded weights.
  *
- * A block in which a key is hidden from one of a wave's queries and not from
- * another goes a key at a time where V there holds infinities or NaNs (0 x inf
- * is NaN), each key for the queries that see it.
+ * Where V holds infinities or NaNs, a key hidden from a query reaches it all the
+ * same (0 x inf is NaN): a workgroup whose outputs are not all finite goes over its
+ * keys again and takes the blocks in which a key is hidden from one of a wave's
+ * queries and not from another a key at a time, each for the queries that see it.
+ * With that beside the loop instead of in it, the loop's registers stay in place:
+ * 8192 and 91 tokens, 32 heads on 8, 627 -> 552 us.
+ *
+ * 550 us there, 1.0 PFLOP/s, is bound by the CU's parts taking turns: a turn of two
+ * workgroups (2.0 us) needs 0.86 of MFMAs, 0.95 of the softmax's VALU and 1.2 of
+ * LDS. 64 sequences of 1 to 1024 tokens take 92: a workgroup of 4.6 turns spends 2
+ * us to find its tile, 3 until its first keys are there, and 2.6 after the last.
+ * Workgroups that go from tile to tile and load the next one's keys in between
+ * needed registers that the loop's values were then moved and spilled for: 116 us,
+ * and 590 for the long one.
  */
 #include "../vx_hip_common.h"
 #include "../vx_packed_kernels.h"
@@ -50,18 +61,13 @@ struct KernelArgs {
   PackedAttnArgs a;
   float scale_log2; /* above 0 */
   uint32_t q_and, q_xor;
-  int group;
+  int group; /* heads of a KV head */
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   const f32x2 v = {lo, hi};
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
-}
-
-/* Not 0 where one of a word's two bf16 is infinite or NaN. */
-__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
-  return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
 /* The lane's number, read again: an address made from it where it is used needs
@@ -124,7 +130,7 @@ struct Tile {
  * more: the index is the highest b for which this exceeds `rank`. More
  * sequences: in the order of the rows. */
 __device__ __forceinline__ Tile tile_of(const PackedAttnArgs &a, int group, int tile, int rank) {
-  const int lane = threadIdx.x & 63;
+  const int lane = lane_here();
   auto tiles = [&](int len) { return (int)(((int64_t)len * group + tile - 1) / tile); };
   if (a.sequences <= kSorted) {
     constexpr int kEach = kSorted / 64;
@@ -217,13 +223,6 @@ __device__ __forceinline__ Tile tile_of(const PackedAttnArgs &a, int group, int 
   return Tile{Span{0, 0}, -1};
 }
 
-/* The last d-step of a query waits in LDS where its registers would be spilled
- * (to memory, whose reload waits for the keys in flight). */
-template <int kD, int kGroups> constexpr bool kParkQ = kD == 128 && kGroups == 1;
-template <int kD, int kGroups> constexpr int lds_bytes() {
-  return 4 * kBK * kD * 2 + (kParkQ<kD, kGroups> ? kThreads * 16 : 0);
-}
-
 /* Tiles of 128 / kGroups rows. */
 template <int kD, int kGroups>
 __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
@@ -239,7 +238,7 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
   constexpr int kDSteps = kD / 16;
   constexpr int kDTiles = kD / 32;
   constexpr int kRowBytes = kD * 2;
-  __shared__ __attribute__((aligned(16))) char lds[lds_bytes<kD, kGroups>()];
+  __shared__ __attribute__((aligned(16))) char lds[4 * kBK * kD * 2];
 
   /* Workgroup i runs on XCD i % 8: where the KV heads are a multiple of 8, each
    * XCD has its own, whose keys its L2 then holds alone. */
@@ -260,14 +259,23 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
   const int keys_all = tile.span.len;
   const int rows_all = keys_all * p.group;
   const int row0 = tile.index * kTileRows;
+  /* the keys that any row of the tile sees, in blocks */
+  const int pos_last = (min(row0 + kTileRows, rows_all) - 1) / p.group;
+  const int turns = ((p.a.causal ? pos_last + 1 : keys_all) + kBK - 1) / kBK;
 
   const int t = threadIdx.x;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int lane = t & 63;
-  const int lq = lane & 31;
   const int g = lane >> 5;
   const int grp = kGroups == 1 ? 0 : wave / kWavesQ;
   const int wq = kGroups == 1 ? wave : wave % kWavesQ;
+
+  /* The lane's number where addresses are made of it: read again, they need no
+   * registers in between, of which 128 rows of 128 have none to spare but for K's
+   * (64 sequences of up to 1024, 32 heads on 8: 95.8 us, with K's kept 92.2, with
+   * all, where values spill, 104; 1 x 512 in 64 rows 15.2, and kept 13.5). */
+  constexpr bool kKeep = kD == 64 || kGroups == 2;
+  auto lane_for = [&] { return kKeep ? lane : lane_here(); };
 
   /* Load l of a thread fills unit l * kGroupThreads + tg of a plane: key row
    * l * kRowsPer + tg / kChunks, whose place differs from l = 0's by an XOR. */
@@ -279,7 +287,7 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
   const uint32_t ring_base = (uint32_t)(uintptr_t)(VX_LDS void *)ring;
   const int kv_bytes = (int)p.a.kv_row * 2; /* from a key to the next */
   const int64_t kv_base = (int64_t)tile.span.begin * p.a.kv_row + kv * p.a.kv_head;
-  /* A group's turn j has block j * kGroups + grp. */
+  /* A group's turn j has block j * kGroups + grp, in slot j % 2. */
   auto key_of = [&](int j) { return (j * kGroups + grp) * kTileKeys; };
   auto issue = [&](int j, int plane) {
     const int key0 = key_of(j);
@@ -288,11 +296,11 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
     const uint16_t *src = plane == 0 ? p.a.k : p.a.v;
     i32x4 rs = buffer_rsrc(src + kv_base + (int64_t)key0 * p.a.kv_row, bytes);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      rs[w] = __builtin_amdgcn_readfirstlane(rs[w]); /* uniform, which the compiler cannot tell */
+    for (int e = 0; e < 4; ++e) {
+      rs[e] = __builtin_amdgcn_readfirstlane(rs[e]); /* uniform, which the compiler cannot tell */
     }
     const uint32_t base = ring_base + (uint32_t)((((j & 1) * 2 + plane) * kUnits + wq * 64) * 16);
-    const uint32_t tg = (uint32_t)(wq * 64 + lane_here());
+    const uint32_t tg = (uint32_t)(wq * 64 + lane_for());
     const int row = (int)(tg / kChunks), c = (int)(tg % kChunks);
     const int place = (plane == 0 ? place_k<kChunks>(row, c) : place_v<kChunks>(row, c)) * 16;
     const int off = row * kv_bytes;
@@ -303,50 +311,46 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
             base + (uint32_t)(l * kGroupThreads * 16));
     }
   };
-
-  /* The keys that any row of the tile sees. The first two blocks of K and the
-   * first of V are on their way before anything else is looked at. */
-  const int pos_last = (min(row0 + kTileRows, rows_all) - 1) / p.group;
-  const int keys_seen = p.a.causal ? pos_last + 1 : keys_all;
-  const int turns = (keys_seen + kBK - 1) / kBK;
+  /* The lane's row: its place and position, and whether it is one (else the
+   * sequence's last). */
+  struct Row {
+    int64_t at;
+    int pos, head;
+    bool real;
+  };
+  auto row_of = [&] {
+    const int r = row0 + 32 * wq + (lane_here() & 31);
+    const int in = min(r, rows_all - 1), pos = in / p.group;
+    return Row{(int64_t)tile.span.begin + pos, pos, kv * p.group + (in - pos * p.group), r < rows_all};
+  };
+  u32x4 qf[kDSteps];
+  auto load_q = [&] {
+    const Row row = row_of();
+    const uint16_t *src = p.a.q + row.at * p.a.q_row + row.head * p.a.q_head + 8 * (lane_here() >> 5);
+#pragma unroll
+    for (int s = 0; s < kDSteps; ++s) {
+      qf[s] = *reinterpret_cast<const u32x4 *>(src + 16 * s);
+    }
+  };
+  /* The first two blocks of K and the first of V are on their way before anything
+   * else is looked at. */
   issue(0, 0);
   issue(0, 1);
   if (turns > 1) {
     issue(1, 0);
   }
+  load_q();
 
-  const int row = row0 + 32 * wq + lq;
-  const bool real = row < rows_all;
-  const int pos = row / p.group;
-  const int head = kv * p.group + (row - pos * p.group);
-  const int64_t at_row = tile.span.begin + pos;
-  u32x4 qf[kDSteps];
-#pragma unroll
-  for (int s = 0; s < kDSteps; ++s) {
-    qf[s] = u32x4{0, 0, 0, 0};
-    if (real) {
-      qf[s] = *reinterpret_cast<const u32x4 *>(p.a.q + at_row * p.a.q_row + head * p.a.q_head +
-                                               8 * g + 16 * s);
-    }
-    /* the scale's sign goes into the query, so that a hidden key's score is -inf
-     * whatever the scale */
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      qf[s][w] = (qf[s][w] & p.q_and) ^ p.q_xor;
-    }
-  }
   /* The last key that each of the wave's rows sees, and all or any of them. */
   const int wave_row = row0 + 32 * wq;
-  const int lim_lo = p.a.causal ? __builtin_amdgcn_readfirstlane(wave_row / p.group) : keys_all - 1;
-  const int lim_hi = wave_row >= rows_all ? -1
-                     : p.a.causal
-                         ? __builtin_amdgcn_readfirstlane(min(wave_row + 31, rows_all - 1) / p.group)
-                         : keys_all - 1;
-  const int limit = real && p.a.causal ? pos : lim_hi;
-  VX_LDS u32x4 *parked = (VX_LDS u32x4 *)(lds + 4 * kBK * kD * 2) + t;
-  if constexpr (kParkQ<kD, kGroups>) {
-    *parked = qf[kDSteps - 1];
-  }
+  const int lim_lo =
+      p.a.causal ? __builtin_amdgcn_readfirstlane(wave_row / p.group) : keys_all - 1;
+  const int lim_hi =
+      wave_row >= rows_all ? -1
+      : p.a.causal
+          ? __builtin_amdgcn_readfirstlane(min(wave_row + 31, rows_all - 1) / p.group)
+          : keys_all - 1;
+  const int limit = p.a.causal ? row_of().pos : keys_all - 1;
 
   /* Where the lane reads in a slot's K plane (row lq, chunk g: chunk 2 ds + g
    * of a place that is an XOR lies at the address XOR 32 ds) and, transposing,
@@ -354,12 +358,12 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
    * 32-wide tile, i = lane % 16, j = lane / 16 % 2, which hands it the 8 keys
    * of its k-slots at d = lane % 32; tile i lies at XOR 64 i. */
   auto keys_at = [&](int j) {
-    const int l = lane_here();
+    const int l = lane;
     return ring_base + (uint32_t)((j & 1) * 2 * kUnits * 16 + (l & 31) * kRowBytes +
                                   place_k<kChunks>(l & 31, l >> 5) * 16);
   };
   auto values_at = [&](int j) {
-    const int l = lane_here();
+    const int l = lane_for();
     const int key = 4 * (l >> 5) + ((l & 15) >> 2);
     const int d = 16 * ((l >> 4) & 1) + 4 * (l & 3);
     return ring_base + (uint32_t)(((j & 1) * 2 + 1) * kUnits * 16 + key * kRowBytes +
@@ -367,23 +371,18 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
   };
 
   f32x16 o[kDTiles];
-#pragma unroll
-  for (int i = 0; i < kDTiles; ++i) {
-    o[i] = f32x16{};
-  }
-  float m_run = -INFINITY, l_run = 0.0f;
+  float m_run, l_run;
 
   typedef f32x16 Scores[kKT];
   auto scores = [&](int j, Scores &st) {
     const uint32_t at = keys_at(j);
 #pragma unroll
     for (int ds = 0; ds < kDSteps; ++ds) {
-      const u32x4 q = kParkQ<kD, kGroups> && ds == kDSteps - 1 ? *parked : qf[ds];
 #pragma unroll
       for (int kt = 0; kt < kKT; ++kt) {
         const u32x4 a = *(const VX_LDS u32x4 *)(uintptr_t)((at ^ (uint32_t)(ds << 5)) +
                                                            (uint32_t)(kt * 32 * kRowBytes));
-        st[kt] = mfma32(a, q, ds == 0 ? f32x16{} : st[kt]);
+        st[kt] = mfma32(a, qf[ds], ds == 0 ? f32x16{} : st[kt]);
       }
     }
   };
@@ -493,6 +492,41 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
     }
   };
 
+  /* What a block hides of a wave's rows: keys past the sequence's last, or past
+   * those that a row sees. */
+  struct Block {
+    int key0, keys; /* from the block's first on */
+    bool hidden, mask;
+  };
+  auto block_of = [&](int j) {
+    const int key0 = key_of(j), keys = keys_all - key0;
+    const bool hidden = key0 + min(keys, kTileKeys) - 1 > lim_lo;
+    return Block{key0, keys, hidden, keys < kTileKeys || hidden};
+  };
+  auto hide = [&](const Block &b, Scores &st) {
+    /* the last key of the block it sees, against constants: keys that are
+     * registers would be kept through the loop, and spilled */
+    const int seen = min(limit - b.key0, b.keys - 1) - 4 * (lane_here() >> 5);
+#pragma unroll
+    for (int kt = 0; kt < kKT; ++kt) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        st[kt][r] = 32 * kt + 8 * (r >> 2) + (r & 3) <= seen ? st[kt][r] : -INFINITY;
+      }
+    }
+  };
+  auto rescale = [&](bool bump, float alpha) {
+    if (__builtin_amdgcn_ballot_w64(bump) != 0) {
+#pragma unroll
+      for (int i = 0; i < kDTiles; ++i) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          o[i][r] *= alpha;
+        }
+      }
+    }
+  };
+
   /* One turn; entering it, K of it and the next and V of it are requested and
    * its scores are in `st`. */
   auto step = [&](int j, Scores &st, Scores &sn) {
@@ -504,18 +538,15 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
     if (j + 1 < turns) {
       issue(j + 1, 1);
     }
-    const int key0 = key_of(j);
-    if (key0 > lim_hi) {
+    const Block b = block_of(j);
+    if (b.key0 > lim_hi) {
       return;
     }
-    const int keys = keys_all - key0; /* from the block's first on */
-    const bool hidden = key0 + min(keys, kTileKeys) - 1 > lim_lo;
-    const bool need_mask = keys < kTileKeys || hidden;
-    const bool next = j + 1 < turns && key_of(j + 1) <= lim_hi;
+    const bool ahead = j + 1 < turns && key_of(j + 1) <= lim_hi;
     u32x4 pt[kKS];
     float alpha;
     bool bump;
-    if (!need_mask && next) {
+    if (!b.mask && ahead) {
       scores(j + 1, sn);
       bump = softmax(st, pt, alpha);
       constexpr int kProducts = kDSteps * kKT, kLead = kProducts >= 16 ? 8 : 4;
@@ -524,56 +555,73 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
       for (int i = 0; i < kProducts; ++i) {
         __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); /* MFMA */
         __builtin_amdgcn_sched_group_barrier(0x002, 6, 0); /* VALU */
-        if (i < kProducts - kLead + (kParkQ<kD, kGroups> ? 1 : 0)) {
+        if (i < kProducts - kLead) {
           __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
         }
       }
     } else {
-      if (next) {
+      if (ahead) {
         scores(j + 1, sn);
       }
-      if (need_mask) {
-        /* the last key of the block it sees, against constants: keys that are
-         * registers would be kept through the loop, and spilled */
-        const int seen = min(limit - key0, keys - 1) - 4 * (lane_here() >> 5);
-#pragma unroll
-        for (int kt = 0; kt < kKT; ++kt) {
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            st[kt][r] = 32 * kt + 8 * (r >> 2) + (r & 3) <= seen ? st[kt][r] : -INFINITY;
-          }
-        }
+      if (b.mask) {
+        hide(b, st);
       }
       bump = softmax(st, pt, alpha);
     }
-    if (__builtin_amdgcn_ballot_w64(bump) != 0) {
-#pragma unroll
-      for (int i = 0; i < kDTiles; ++i) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          o[i][r] *= alpha;
-        }
-      }
-    }
-    if (hidden) {
-      uint32_t any = 0;
-      const uint32_t at = values_at(j);
-#pragma unroll 1
-      for (int ks = 0; ks < kKS; ++ks) {
-#pragma unroll
-        for (int i = 0; i < kDTiles; ++i) {
-          const u32x4 a = values(at, ks, i);
-          any |= not_finite(a[0]) | not_finite(a[1]) | not_finite(a[2]) | not_finite(a[3]);
-        }
-      }
-      if (__builtin_amdgcn_ballot_w64(any != 0) != 0) {
-        accumulate_apart(j, pt, min(limit - key0, keys - 1));
-        return;
-      }
-    }
+    rescale(bump, alpha);
     accumulate(j, pt);
   };
+  /* The tile's queries, loaded, as scores() takes them; and nothing seen yet. */
+  auto start = [&] {
+#pragma unroll
+    for (int s = 0; s < kDSteps; ++s) {
+      /* the scale's sign goes into the query, so that a hidden key's score is -inf
+       * whatever the scale */
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        qf[s][e] = (qf[s][e] & p.q_and) ^ p.q_xor;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kDTiles; ++i) {
+      o[i] = f32x16{};
+    }
+    m_run = -INFINITY;
+    l_run = 0.0f;
+  };
+  /* The tile over again, a block at a time. */
+  auto carefully = [&] {
+    load_q();
+    start();
+#pragma unroll 1
+    for (int j = 0; j < turns; ++j) {
+      lds_barrier();
+      issue(j, 0);
+      issue(j, 1);
+      wait_vm<0>();
+      lds_barrier();
+      const Block b = block_of(j);
+      if (b.key0 > lim_hi) {
+        continue;
+      }
+      Scores st;
+      scores(j, st);
+      if (b.mask) {
+        hide(b, st);
+      }
+      u32x4 pt[kKS];
+      float alpha;
+      const bool bump = softmax(st, pt, alpha);
+      rescale(bump, alpha);
+      if (b.hidden) {
+        accumulate_apart(j, pt, min(limit - b.key0, b.keys - 1));
+      } else {
+        accumulate(j, pt);
+      }
+    }
+  };
 
+  start();
   Scores sa, sb;
   wait_vm<0>();
   lds_barrier();
@@ -584,6 +632,20 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
     step(j, sa, sb);
     if (j + 1 < turns) {
       step(j + 1, sb, sa);
+    }
+  }
+  if (p.a.causal) {
+    /* x 0 is NaN of what is not finite */
+    float zero = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kDTiles; ++i) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        zero = __builtin_fmaf(o[i][r], 0.0f, zero);
+      }
+    }
+    if (__syncthreads_or(zero != zero)) {
+      carefully();
     }
   }
 
@@ -626,24 +688,24 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
       }
     }
   }
-  if (!real) {
-    return;
-  }
-  const bool seen = m_run > -INFINITY || l_run != 0.0f;
-  const float inv = seen ? 1.0f / l_run : 0.0f;
-  uint16_t *dst = p.a.o + at_row * p.a.o_row + head * p.a.o_head;
+  const Row row = row_of();
+  if (row.real) {
+    const bool seen = m_run > -INFINITY || l_run != 0.0f;
+    const float inv = seen ? 1.0f / l_run : 0.0f;
+    uint16_t *dst = p.a.o + row.at * p.a.o_row + row.head * p.a.o_head;
 #pragma unroll
-  for (int i = 0; i < kDTiles; ++i) {
+    for (int i = 0; i < kDTiles; ++i) {
 #pragma unroll
-    for (int r4 = 0; r4 < 4; ++r4) {
-      *reinterpret_cast<u32x2 *>(dst + 32 * i + 8 * r4 + 4 * g) =
-          u32x2{pack2(o[i][4 * r4] * inv, o[i][4 * r4 + 1] * inv),
-                pack2(o[i][4 * r4 + 2] * inv, o[i][4 * r4 + 3] * inv)};
+      for (int r4 = 0; r4 < 4; ++r4) {
+        *reinterpret_cast<u32x2 *>(dst + 32 * i + 8 * r4 + 4 * g) =
+            u32x2{pack2(o[i][4 * r4] * inv, o[i][4 * r4 + 1] * inv),
+                  pack2(o[i][4 * r4 + 2] * inv, o[i][4 * r4 + 3] * inv)};
+      }
     }
-  }
-  if (p.a.lse && g == 0) {
-    p.a.lse[(int64_t)head * p.a.total + at_row] =
-        seen ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+    if (p.a.lse && g == 0) {
+      p.a.lse[(int64_t)row.head * p.a.total + row.at] =
+          seen ? (m_run + log2f(l_run)) * kLn2 : -INFINITY;
+    }
   }
 }
 
