@@ -274,3 +274,13 @@ def test_from_a_graph_on_another_stream(hiplib):
         t.stream_destroy(stream_)
     c.check()
     c.free()
+
+
+@pytest.mark.parametrize("dtype,rows,dim", [("bf16", 2100, 4096), ("f32", 1100, 4096), ("bf16", 5000, 3600)])
+def test_inputs_past_the_caches(hiplib, dtype, rows, dim):
+    announce(f"rms_norm past the caches {rows} x {dim} {dtype}")
+    rng = np.random.default_rng(12)
+    c = Call(hiplib, dtype, stream(rng, rows, dim), stream(rng, rows, dim), rng.standard_normal(dim), ("sum", "y", "q"))
+    c()
+    c.check()
+    c.free()

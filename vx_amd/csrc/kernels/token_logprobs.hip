@@ -64,6 +64,21 @@ __device__ __forceinline__ Sums against(Sums v, float top) {
   return v.s > 0.0f ? Sums{top, v.s * f, f * (v.e + v.s * d)} : Sums{top, 0.0f, 0.0f};
 }
 
+__device__ __forceinline__ u64 wave_min_key(u64 v) {
+  auto meet = [&](auto step) {
+    constexpr int kO = decltype(step)::value;
+    const u64 o = (u64)partner_word<kO>((u32)(v >> 32)) << 32 | partner_word<kO>((u32)v);
+    v = min(v, o);
+  };
+  meet(std::integral_constant<int, 1>{});
+  meet(std::integral_constant<int, 2>{});
+  meet(std::integral_constant<int, 4>{});
+  meet(std::integral_constant<int, 8>{});
+  meet(std::integral_constant<int, 16>{});
+  meet(std::integral_constant<int, 32>{});
+  return v;
+}
+
 template <bool kF32> struct Elements {
   static constexpr int kVec = kF32 ? 4 : 8; /* of a 16-byte load */
   const void *row;
@@ -313,7 +328,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(LogprobArgs a, Logprob
       }
       return c;
     };
-    u64 lo = 1, hi = key_of(top, 0) + 1; /* from(lo) >= n > from(hi), if any */
+    /* from(lo) >= n > from(hi), if there are n: all from the least on */
+    u64 lo = k[0], hi = key_of(top, 0) + 1;
+#pragma unroll
+    for (int i = 1; i < kWaves; ++i) {
+      lo = min(lo, k[i]);
+    }
+    lo = max(wave_min_key(lo), (u64)1);
     int c = from(lo);
     while (c > 64) {
       const u64 mid = lo + (hi - lo) / 2;
@@ -358,18 +379,21 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(LogprobArgs a, Logprob
         }
       }
     };
-    for (int c = wave; c < threads; c += kWaves) {
-      const int owner = sh.which[c];
-      if (owner < singles && lane == 0) {
-        const int at = owner < lead - begin ? begin + owner : tail + (owner - (lead - begin));
-        add(key_of(x.at(at), at));
-      }
-      for (int i = owner + lane * kThreads; i < vectors; i += 64 * kThreads) {
-        float v[kVec];
-        Elements<kF32>::open(x.raw(lead + (int64_t)i * kVec), v);
+    if (t < threads && sh.which[t] < singles) {
+      const int owner = sh.which[t];
+      const int at = owner < lead - begin ? begin + owner : tail + (owner - (lead - begin));
+      add(key_of(x.at(at), at));
+    }
+    /* every vector of theirs, a thread one at a time */
+    const int per = (vectors + kThreads - 1) / kThreads;
+    for (int i = t; i < per * threads; i += kThreads) {
+      const int v = sh.which[i % threads] + i / threads * kThreads;
+      if (v < vectors) {
+        float el[kVec];
+        Elements<kF32>::open(x.raw(lead + (int64_t)v * kVec), el);
 #pragma unroll
-        for (int el = 0; el < kVec; ++el) {
-          add(key_of(v[el], lead + i * kVec + el));
+        for (int j = 0; j < kVec; ++j) {
+          add(key_of(el[j], lead + v * kVec + j));
         }
       }
     }
