@@ -90,16 +90,17 @@ def token_logprobs(logits, given, n_top):
     """float64 (logprob, entropy, top_tokens, top_logprob) of float logits, and
     the bounds of the three that are computed.
 
-    A thread sums up to e = max(32, vocab / 1024) + 8 weights in f32, each e^d off
-    by 2^-23 (|d| + 2), against a reference up to 8 below its logits, and some 40
-    roundings join the threads' sums."""
+    A thread sums up to e = max(96, vocab / 1024) + 8 weights in f32 (rows of up to
+    2048, 4096, 12288 and 49152 have 64, 128, 256 and 512 threads, longer ones
+    1024), each e^d off by 2^-23 (|d| + 2), against a reference up to 8 below its
+    logits, and some 40 roundings join the threads' sums."""
     x = logits.astype(np.float64)
     x = np.where(np.isnan(x), -np.inf, x)
     rows, vocab = x.shape
     logprob, entropy = np.full(given.shape, -np.inf), np.zeros(rows)
     top_tokens, top_logprob = np.full((rows, n_top), -1, np.int32), np.full((rows, n_top), -np.inf)
     tol = [np.zeros(a.shape) for a in (logprob, entropy, top_logprob)]
-    each = max(32, vocab / 1024) + 8 + 40
+    each = max(96, vocab / 1024) + 8 + 40
     for r in range(rows):
         top = x[r].max()
         if top == -np.inf:

@@ -16,6 +16,11 @@
  *
  * Rows fewer than CUs are divided: a workgroup a slice leaves its sums and its
  * likeliest in a workspace, logprobs_merge adds them up.
+ *
+ * 512 x 131071 bf16 with entropy and 20 alternatives 36 us, of which 31 without
+ * alternatives (4.35 TB/s: the row's reading bounds it), 2048 x 32000 f32 44 (5.9
+ * TB/s) and 55 with 5 alternatives. 1 x 32000 9.1: 5.8 for the sums, of which half
+ * the launch, and 3.3 for the alternatives, a chain of barriers and two loads.
  */
 #include "../vx_hip_common.h"
 #include "../vx_packed_kernels.h"
@@ -35,7 +40,6 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;
 constexpr int kMostTop = 64;
-constexpr int kList = 2048;
 
 /* Rises with l; 0 for -inf and NaN, which are no alternatives. */
 __device__ __forceinline__ u32 order_of(float l) {
@@ -126,6 +130,7 @@ struct Part {
 
 template <int kThreads> struct Shared {
   static constexpr int kWaves = kThreads / 64;
+  static constexpr int kList = kThreads < 256 ? 8 * kThreads : 2048; /* above 64 */
   float a[kWaves], b[kWaves];
   int n[kWaves];
   u64 best[kThreads];
@@ -135,16 +140,22 @@ template <int kThreads> struct Shared {
 };
 
 /* The n largest keys of the list, in falling order, to `put`; what is not there
- * is 0. */
+ * is 0. Eight lanes compare a key with an eighth of the others each. */
 template <int kThreads, typename Put>
 __device__ __forceinline__ void in_order(const u64 *list, int count, int n, Put put) {
-  for (int i = threadIdx.x; i < count; i += kThreads) {
-    const u64 mine = list[i];
+  const int part = threadIdx.x & 7;
+  for (int i0 = 0; i0 < count; i0 += kThreads / 8) {
+    const int i = i0 + (int)threadIdx.x / 8;
+    const u64 mine = list[min(i, count - 1)];
     int above = 0;
-    for (int j = 0; j < count; ++j) {
+#pragma unroll 4
+    for (int j = part; j < count; j += 8) {
       above += list[j] > mine;
     }
-    if (above < n) {
+    above += (int)partner_word<1>((u32)above);
+    above += (int)partner_word<2>((u32)above);
+    above += (int)partner_word<4>((u32)above);
+    if (part == 0 && i < count && above < n) {
       put(above, mine);
     }
   }
@@ -172,6 +183,7 @@ template <bool kF32, int kThreads, bool kSliced>
 __global__ __launch_bounds__(kThreads) void logprobs_rows(LogprobArgs a, LogprobPlan plan, Part *parts) {
   constexpr int kVec = Elements<kF32>::kVec;
   constexpr int kWaves = kThreads / 64;
+  constexpr int kList = Shared<kThreads>::kList;
   __shared__ Shared<kThreads> sh;
   const int t = threadIdx.x;
   const int lane = t & 63;
@@ -312,8 +324,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(LogprobArgs a, Logprob
     return;
   }
 
-  /* A border with at least n threads' largest at or above it and at most 64 (or
-   * all, where there are no n): one wave halves the keys' range. */
+  /* A border with at least n threads' largest at or above it and not many more
+   * (or all, where there are no n): one wave halves the keys' range. */
   if (wave == 0) {
     u64 k[kWaves];
 #pragma unroll
@@ -336,7 +348,8 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(LogprobArgs a, Logprob
     }
     lo = max(wave_min_key(lo), (u64)1);
     int c = from(lo);
-    while (c > 64) {
+    const int most = max(n, kThreads / 16);
+    while (c > most) {
       const u64 mid = lo + (hi - lo) / 2;
       const int m = from(mid);
       if (m >= n) {
@@ -431,26 +444,36 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(LogprobArgs a, Logprob
 }
 
 constexpr int kMergeThreads = 256;
-constexpr int kMostSlices = 64;
+constexpr int kMostSlices = 16;
 
 __global__ __launch_bounds__(kMergeThreads) void logprobs_merge(LogprobArgs a, LogprobPlan plan,
                                                                const Part *parts) {
   __shared__ u64 list[kMostSlices * kMostTop];
+  __shared__ int real;
   const int64_t r = blockIdx.x;
   const Part *mine = parts + r * plan.slices;
-  float top = -INFINITY;
-  int infs = 0;
-  for (int i = 0; i < plan.slices; ++i) {
-    top = fmaxf(top, mine[i].top);
-    infs += mine[i].infs;
+  const int n = a.n_top, all = n * plan.slices;
+  if (threadIdx.x == 0) {
+    real = 0;
   }
+  __syncthreads();
+  /* keys of 0 are none */
+  for (int i = threadIdx.x; i < all; i += kMergeThreads) {
+    const u64 key = mine[i / n].keys[i % n];
+    if (key) {
+      list[atomicAdd(&real, 1)] = key;
+    }
+  }
+  /* a lane a slice, on every wave */
+  const int lane = threadIdx.x & 63;
+  const bool has = lane < plan.slices;
+  const Part &part = mine[min(lane, plan.slices - 1)];
+  const Sums own{part.top, part.s, part.e};
+  const float top = wave_max(own.m);
+  const int infs = wave_sum_int(has ? part.infs : 0);
   const bool none = !(top > -INFINITY), inf = top == INFINITY;
-  float s = 0.0f, e = 0.0f;
-  for (int i = 0; i < plan.slices && !none && !inf; ++i) {
-    const Sums v = against(Sums{mine[i].top, mine[i].s, mine[i].e}, top);
-    s += v.s;
-    e += v.e;
-  }
+  const Sums v = has && !none && !inf ? against(own, top) : Sums{0.0f, 0.0f, 0.0f};
+  const float s = wave_sum(v.s), e = wave_sum(v.e);
   Row row{top, 0.0f, 0.0f, inf};
   row.log_sum = inf ? logf((float)infs) : none ? 0.0f : logf(s);
   row.entropy = inf ? row.log_sum : none ? 0.0f : fmaxf(row.log_sum - e / s, 0.0f);
@@ -458,57 +481,56 @@ __global__ __launch_bounds__(kMergeThreads) void logprobs_merge(LogprobArgs a, L
   if (a.entropy && threadIdx.x == 0) {
     a.entropy[r] = row.entropy;
   }
-  const int n = a.n_top, all = n * plan.slices;
-  for (int i = threadIdx.x; i < all; i += kMergeThreads) {
-    list[i] = mine[i / n].keys[i % n];
-  }
   __syncthreads();
-  /* keys of 0 are none and may be many: only the others are written */
-  for (int i = threadIdx.x; i < all; i += kMergeThreads) {
-    const u64 key = list[i];
-    int above = 0;
-    for (int j = 0; j < all; ++j) {
-      above += list[j] > key;
-    }
-    if (key && above < n) {
-      a.top_tokens[r * n + above] = index_of(key);
-      if (a.top_logprob) {
-        a.top_logprob[r * n + above] = logprob_of(row, logit_of(key));
-      }
-    }
-  }
-  int real = 0;
-  for (int j = 0; j < all; ++j) {
-    real += list[j] != 0;
-  }
-  for (int i = real + threadIdx.x; i < n; i += kMergeThreads) {
-    a.top_tokens[r * n + i] = -1;
+  in_order<kMergeThreads>(list, real, n, [&](int i, u64 key) {
+    a.top_tokens[r * n + i] = key ? index_of(key) : -1;
     if (a.top_logprob) {
-      a.top_logprob[r * n + i] = -INFINITY;
+      a.top_logprob[r * n + i] = key ? logprob_of(row, logit_of(key)) : -INFINITY;
     }
-  }
+  });
 }
 
+template <bool kF32, int kThreads>
+void launch_rows(const LogprobArgs &a, const LogprobPlan &plan, hipStream_t stream) {
+  hipLaunchKernelGGL((logprobs_rows<kF32, kThreads, false>), dim3((unsigned)a.rows), dim3(kThreads), 0,
+                     stream, a, plan, nullptr);
+}
+
+/* Threads by the row's length, in us: 4096 x 1000 9.0 by 64, 14.9 by 256; 4096 x
+ * 4000 18.7 by 128, 19.9 by 64; 4096 x 8000 34 by 256, 39 by 128 or 512; 2048 x
+ * 32000 55 by 512, 60 by 1024; 512 x 131071 37 by 1024, 41 by 512. */
 template <bool kF32>
 void launch(const LogprobArgs &a, const LogprobPlan &plan, Part *parts, hipStream_t stream) {
   const dim3 grid((unsigned)((int64_t)a.rows * plan.slices));
   if (plan.slices > 1) {
-    hipLaunchKernelGGL((logprobs_rows<kF32, 1024, true>), grid, dim3(1024), 0, stream, a, plan, parts);
+    hipLaunchKernelGGL((logprobs_rows<kF32, 512, true>), grid, dim3(512), 0, stream, a, plan, parts);
     hipLaunchKernelGGL(logprobs_merge, dim3((unsigned)a.rows), dim3(kMergeThreads), 0, stream, a, plan,
                        parts);
-  } else if (a.vocab <= 8192) {
-    hipLaunchKernelGGL((logprobs_rows<kF32, 256, false>), grid, dim3(256), 0, stream, a, plan, parts);
+  } else if (a.vocab <= 2048) {
+    launch_rows<kF32, 64>(a, plan, stream);
+  } else if (a.vocab <= 4096) {
+    launch_rows<kF32, 128>(a, plan, stream);
+  } else if (a.vocab <= 12288) {
+    launch_rows<kF32, 256>(a, plan, stream);
+  } else if (a.vocab <= 49152) {
+    launch_rows<kF32, 512>(a, plan, stream);
   } else {
-    hipLaunchKernelGGL((logprobs_rows<kF32, 1024, false>), grid, dim3(1024), 0, stream, a, plan, parts);
+    launch_rows<kF32, 1024>(a, plan, stream);
   }
 }
 
 } // namespace
 
+/* Slices of a row: as many as give 256 workgroups, of at least 12288 logits, and
+ * with no more than 160 alternatives in all, which the merge compares each with
+ * each. In us, undivided and in 2, 4, 8 and 16: 1 x 131072 with 5 alternatives 18,
+ * 16.2, 11.8, 10.3 and 10.2; 1 x 50257 10.8, 10.8, 9.7, 9.6 and 10.4; 16 x 131072
+ * with 20 17.7, 15.3, 13.2, 13.3 and 19.9; 64 rows 20.2, 19.4, 15.7, 17.2 and 25;
+ * 128 rows 22.2, 21.5, 20.7, 22.9 and 32. */
 LogprobPlan logprobs_plan(int64_t rows, int64_t vocab, int64_t n_top, bool may_split) {
-  (void)n_top;
   LogprobPlan p{1, (int)vocab, 0};
-  const int64_t want = std::min<int64_t>({256 / rows, vocab / 16384, kMostSlices});
+  const int64_t want = std::min<int64_t>(
+      {256 / rows, vocab / 12288, kMostSlices, 160 / std::max<int64_t>(n_top, 1)});
   if (may_split && want > 1) {
     p.slice = (int)(((vocab + want - 1) / want + 63) / 64 * 64);
     p.slices = (int)((vocab + p.slice - 1) / p.slice);
