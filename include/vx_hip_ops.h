@@ -289,7 +289,7 @@ int64_t vx_nn_gemm_i8_workspace(int64_t tokens, int64_t rows, int64_t cols);
  * Numerics, `scale` and what hidden keys may hold as in
  * vx_nn_flash_attention_shared_bf16. head_dim 64 or 128; strides multiples of 8,
  * at least head_dim; kv_row at most 2^22; pointers 16-byte aligned; at most
- * 65536 sequences and 2^28 queries of all heads. */
+ * 65536 sequences, 2^22 sequences * kv_heads and 2^28 queries of all heads. */
 int32_t vx_nn_flash_attention_packed_bf16(
     const uint16_t *q, const uint16_t *k, const uint16_t *v,
     const int32_t *offsets, uint16_t *o, float *lse, int64_t total,

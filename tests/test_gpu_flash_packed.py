@@ -127,11 +127,21 @@ def test_tiles_of_128_rows(hiplib, d, causal):
 
 @pytest.mark.parametrize("n", [64, 65, 255, 256, 257, 300, 1000, 5000])
 def test_many_sequences(hiplib, n):
-    """Past 256 sequences tiles go in the order of the rows."""
+    """Sequences are searched 64 at a time."""
     rng = np.random.default_rng(n)
     lens = rng.integers(0, 6, n)
     lens[n // 2], lens[n - 1] = 150, 70
     one(hiplib, lens, 3, 1, 64, tail=2, layout="tokens")
+
+
+@pytest.mark.parametrize("heads,kv,d", [(5, 1, 128), (32, 8, 64), (16, 8, 128)])
+def test_many_sequences_of_several_heads(hiplib, heads, kv, d):
+    """Rows before the first sequence, empty ones at both ends, tiles of both
+    sizes."""
+    rng = np.random.default_rng(heads)
+    lens = rng.integers(0, 12, 700)
+    lens[:3], lens[300], lens[-3:] = 0, 190, 0
+    one(hiplib, lens, heads, kv, d, lead=137, tail=40)
 
 
 def test_one_long_sequence_of_one_head(hiplib):
@@ -182,6 +192,22 @@ def test_offsets_that_fall_or_lie_outside_touch_nothing_else(hiplib):
     c.off = DeviceArray.of(hiplib, np.array([-5, 20, 50, 1000], np.int32), abi.DTYPE_I32)
     c()
     c.check(offsets=[0, 20, 50, 60])
+    c.free()
+
+
+def test_many_offsets_that_fall_touch_nothing_else(hiplib):
+    """In any order: rows of no sequence stay."""
+    announce("flash_packed many offsets that fall")
+    n = 900
+    c = Call(hiplib, [2] * n, 4, 2, 64, tail=50)
+    rng = np.random.default_rng(1)
+    for offsets in (rng.permutation(c.offsets), c.offsets[::-1].copy(),
+                    rng.integers(-2 ** 31, 2 * n, n + 1).astype(np.int32)):
+        c.off.free()
+        c.off = DeviceArray.of(hiplib, offsets, abi.DTYPE_I32)
+        c()
+        o, lse = c.outputs()
+        assert np.all(o[:, 2 * n:] == 0x5a5a) and np.all(lse[:, 2 * n:] == 77.5)
     c.free()
 
 

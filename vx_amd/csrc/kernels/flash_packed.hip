@@ -7,9 +7,9 @@
  * each the heads that read one KV head, so that a tile of 128 rows covers 128 /
  * group positions: K and V are read once for all heads of the group, and short
  * sequences fill a tile. Workgroups find their tile from the offsets
- * themselves (tile_of), heaviest tiles first; the launch has as many as there
- * can be tiles, the others end at once. So a captured launch follows the
- * offsets in GPU memory, and no workspace is needed.
+ * themselves (tile_of); the launch has as many as there can be tiles, the others
+ * end at once. So a captured launch follows the offsets in GPU memory, and no
+ * workspace is needed.
  *
  * 4 waves; K and V through a two-slot LDS ring by buffer-to-LDS loads; as in
  * flash_attn.hip the products are transposed, S^T = K Q^T and O^T += V^T P^T
@@ -29,7 +29,7 @@
  *
  * 550 us there, 1.0 PFLOP/s, is bound by the CU's parts taking turns: a turn of two
  * workgroups (2.0 us) needs 0.86 of MFMAs, 0.95 of the softmax's VALU and 1.2 of
- * LDS. 64 sequences of 1 to 1024 tokens take 92: a workgroup of 4.6 turns spends 2
+ * LDS. 64 sequences of 1 to 1024 tokens take 90: a workgroup of 4.6 turns spends 2
  * us to find its tile, 3 until its first keys are there, and 2.6 after the last.
  * Workgroups that go from tile to tile and load the next one's keys in between
  * needed registers that the loop's values were then moved and spilled for: 116 us,
@@ -55,13 +55,13 @@ constexpr int kThreads = 256;
 constexpr int kBK = 64;        /* keys per turn of a workgroup */
 constexpr float kSlack = 8.0f; /* base-2 headroom of the stale row max */
 constexpr float kLn2 = 0.69314718055994531f;
-constexpr int kSorted = 256;   /* sequences whose tiles go heaviest first */
 
 struct KernelArgs {
   PackedAttnArgs a;
   float scale_log2; /* above 0 */
   uint32_t q_and, q_xor;
   int group; /* heads of a KV head */
+  bool sorted;
 };
 
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -124,33 +124,21 @@ struct Tile {
   int index; /* of the sequence's tiles; -1: none */
 };
 
-/* The launch's tile number `rank`, the same on every lane. Up to 256
- * sequences: tiles of the highest index, which see the most keys, come first.
+/* The launch's tile number `rank`, the same on every lane. `sorted`, for at most
+ * 64 sequences: tiles of the highest index, which see the most keys, come first.
  * With n_s tiles in sequence s, sum max(n_s - b, 0) of them have an index of b or
- * more: the index is the highest b for which this exceeds `rank`. More
- * sequences: in the order of the rows. */
-__device__ __forceinline__ Tile tile_of(const PackedAttnArgs &a, int group, int tile, int rank) {
+ * more: the index is the highest b for which this exceeds `rank`. Else in the order
+ * of the sequences, which read their keys at about the same time, each from its last
+ * tile to its first; sequence s from floor(first row / rows of a tile) + s on, which
+ * leaves each at least its tiles and is searched, not added up. */
+__device__ __forceinline__ Tile tile_of(const PackedAttnArgs &a, int group, int tile, int rank,
+                                        bool sorted) {
   const int lane = lane_here();
   auto tiles = [&](int len) { return (int)(((int64_t)len * group + tile - 1) / tile); };
-  if (a.sequences <= kSorted) {
-    constexpr int kEach = kSorted / 64;
-    Span span[kEach];
-    int n[kEach], most = 0;
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int s = e * 64 + lane;
-      span[e] = s < a.sequences ? span_of(a, s) : Span{0, 0};
-      n[e] = tiles(span[e].len);
-      most = max(most, n[e]);
-    }
-    auto from = [&](int b) {
-      int v = 0;
-#pragma unroll
-      for (int e = 0; e < kEach; ++e) {
-        v += max(n[e] - b, 0);
-      }
-      return wave_sum_int(v);
-    };
+  if (sorted) {
+    const Span span = lane < a.sequences ? span_of(a, lane) : Span{0, 0};
+    const int n = tiles(span.len);
+    auto from = [&](int b) { return wave_sum_int(max(n - b, 0)); };
     if (from(0) <= rank) {
       return Tile{Span{0, 0}, -1};
     }
@@ -167,60 +155,32 @@ __device__ __forceinline__ Tile tile_of(const PackedAttnArgs &a, int group, int 
         hi = mid;
       }
     }
-    int j = rank - from(lo + 1); /* among the sequences that have a tile `lo` */
-    Tile t{Span{0, 0}, -1};
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const uint64_t has = __builtin_amdgcn_ballot_w64(n[e] > lo);
-      const int count = __builtin_popcountll(has);
-      if (t.index < 0 && j < count) {
-        const bool me = n[e] > lo && __builtin_popcountll(has & ((1ull << lane) - 1)) == j;
-        const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(me));
-        t = Tile{Span{__builtin_amdgcn_readlane(span[e].begin, who),
-                      __builtin_amdgcn_readlane(span[e].len, who)},
-                 lo};
-      }
-      j -= count;
-    }
-    return t;
+    const int j = rank - from(lo + 1); /* among the sequences that have a tile `lo` */
+    const uint64_t has = __builtin_amdgcn_ballot_w64(n > lo);
+    const bool me = n > lo && __builtin_popcountll(has & ((1ull << lane) - 1)) == j;
+    const int who = __builtin_ctzll(__builtin_amdgcn_ballot_w64(me));
+    return Tile{Span{__builtin_amdgcn_readlane(span.begin, who),
+                     __builtin_amdgcn_readlane(span.len, who)},
+                lo};
   }
-  auto upto = [&](int v) { /* sum over the lanes up to this one */
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int w = __shfl_up(v, o);
-      v += lane >= o ? w : 0;
-    }
-    return v;
+  /* the last sequence that starts at `rank` or before: 64 of them, then 64 in between */
+  auto first = [&](int s) {
+    const int64_t row = min(max(a.offsets[s], 0), a.total);
+    return (int)(row * group / tile) + s;
   };
-  /* each lane a run of the sequences, then the run's, 64 at a time */
-  const int per = (a.sequences + 63) / 64;
-  int mine = 0;
-  for (int i = 0; i < per; ++i) {
-    const int s = lane * per + i;
-    mine += s < a.sequences ? tiles(span_of(a, s).len) : 0;
+  int at = 0;
+  for (int n = a.sequences; n > 1;) { /* it is one of the n from `at` */
+    const int step = (n + 63) / 64;
+    const int s = at + lane * step;
+    const bool past = lane * step >= n || first(min(s, a.sequences - 1)) > rank;
+    const int before = 64 - __builtin_popcountll(__builtin_amdgcn_ballot_w64(past));
+    const int skip = max(before - 1, 0) * step;
+    at += skip;
+    n = min(step, n - skip);
   }
-  const int sum = upto(mine);
-  const uint64_t past = __builtin_amdgcn_ballot_w64(sum > rank);
-  if (past == 0) {
-    return Tile{Span{0, 0}, -1};
-  }
-  const int run = __builtin_ctzll(past);
-  int left = rank - __builtin_amdgcn_readlane(sum - mine, run);
-  for (int i0 = 0; i0 < per; i0 += 64) {
-    const int s = run * per + i0 + lane;
-    const Span span = i0 + lane < per && s < a.sequences ? span_of(a, s) : Span{0, 0};
-    const int n = tiles(span.len);
-    const int until = upto(n);
-    const uint64_t here = __builtin_amdgcn_ballot_w64(until > left);
-    if (here) {
-      const int who = __builtin_ctzll(here);
-      return Tile{Span{__builtin_amdgcn_readlane(span.begin, who),
-                       __builtin_amdgcn_readlane(span.len, who)},
-                  left - __builtin_amdgcn_readlane(until - n, who)};
-    }
-    left -= __builtin_amdgcn_readlane(until, 63);
-  }
-  return Tile{Span{0, 0}, -1};
+  const Span span = span_of(a, at);
+  const int n = tiles(span.len), index = n - 1 - (rank - first(at));
+  return Tile{span, index < n ? index : -1};
 }
 
 /* Tiles of 128 / kGroups rows. */
@@ -252,7 +212,7 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
     rank = (int)blockIdx.x / kv_heads;
     kv = (int)blockIdx.x - rank * kv_heads;
   }
-  const Tile tile = tile_of(p.a, p.group, kTileRows, rank);
+  const Tile tile = tile_of(p.a, p.group, kTileRows, rank, p.sorted);
   if (tile.index < 0) {
     return;
   }
@@ -709,11 +669,20 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
   }
 }
 
-template <int kD, int kGroups> void launch(const KernelArgs &p, hipStream_t stream) {
+template <int kD, int kGroups> void launch(KernelArgs p, hipStream_t stream) {
   constexpr int kTileRows = 128 / kGroups;
-  const int64_t most = (int64_t)p.a.total * p.group / kTileRows + p.a.sequences;
-  hipLaunchKernelGGL((flash_packed<kD, kGroups>), dim3((unsigned)(most * p.a.kv_heads)),
-                     dim3(kThreads), 0, stream, p);
+  const int64_t workgroups =
+      ((int64_t)p.a.total * p.group / kTileRows + p.a.sequences) * p.a.kv_heads;
+  /* Two fit on a CU. Heaviest first ends evenly where they come in a few rounds: 30
+   * sequences of up to 500, 8 heads on 1, 500 workgroups, 19.6 us, in the sequences'
+   * order 22.5; 64 of up to 300, 12 heads, 1670, 40.5 and 43.6; 64 of up to 1024, 32
+   * on 8, 3000, 89.9 and 92.7. In one round the search costs more than it gains (8 of
+   * up to 260, 32 on 8, tiles of 64 rows, 16.2 and 14.7), in many the keys of other
+   * sequences in between (64 of up to 1024, 12 heads, 3830, 146 and 137; 32 on 8,
+   * 8760, 309 and 284). */
+  p.sorted = kGroups == 1 && p.a.sequences <= 64 && workgroups <= 12 * (int64_t)device_cu_count();
+  hipLaunchKernelGGL((flash_packed<kD, kGroups>), dim3((unsigned)workgroups), dim3(kThreads), 0,
+                     stream, p);
 }
 
 } // namespace
@@ -726,9 +695,13 @@ void flash_packed_launch(const PackedAttnArgs &a, int head_dim, hipStream_t stre
   p.scale_log2 = a.scale != 0.0f ? std::fabs(a.scale) * 1.4426950408889634f : 1.0f;
   p.q_and = a.scale != 0.0f ? 0xffffffffu : 0u;
   p.q_xor = a.scale < 0.0f ? 0x80008000u : 0u;
-  /* two groups where workgroups of 128 rows would leave CUs idle */
+  /* Tiles of 64 rows, whose keys two halves of the workgroup divide, where those of
+   * 128 would be few: 1 sequence of 1000, 12 heads (108 workgroups) 18.8 us, in tiles
+   * of 128 25.9; 1 of 4000 (384) 67.6 and 80.7; 20 of up to 1000 (444) 21.5 and 27.6;
+   * but 1 of 1800, 32 heads on 8 (456), 47.3 and 44.4, and 1 of 2500 (632) 77.5 and
+   * 68.6. Half of the tiles of one row that many sequences may need are counted. */
   const int64_t wide = ((int64_t)a.total * p.group / 128 + (a.sequences + 1) / 2) * a.kv_heads;
-  const bool two = wide < device_cu_count();
+  const bool two = 4 * wide < 7 * (int64_t)device_cu_count();
   if (head_dim == 64) {
     two ? launch<64, 2>(p, stream) : launch<64, 1>(p, stream);
   } else {

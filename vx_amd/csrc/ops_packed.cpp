@@ -223,13 +223,13 @@ int32_t vx_nn_flash_attention_packed_bf16(const uint16_t *q, const uint16_t *k, 
       return refuse(VX_OP_EUNSUPP, op, "strides must be multiples of 8");
     }
   }
-  /* Rows of a sequence's queries, workgroups, and byte offsets within a block of
-   * keys are 31-bit. */
+  /* Rows of a sequence's queries, threads of a launch, and byte offsets within a
+   * block of keys are 31-bit. */
   const int64_t rows = product({total, heads});
-  if (rows < 0 || rows > INT32_MAX / 2 || sequences > 65536 ||
-      (rows / 64 + sequences * kv_heads) > (int64_t(1) << 23) || kv_row > (int64_t(1) << 22)) {
-    return refuse(VX_OP_EUNSUPP, op, "more than 2^28 queries of all heads or 65536 sequences, or "
-                                     "kv_row above 2^22");
+  if (rows < 0 || rows > (int64_t(1) << 28) || sequences > 65536 ||
+      sequences * kv_heads > (int64_t(1) << 22) || kv_row > (int64_t(1) << 22)) {
+    return refuse(VX_OP_EUNSUPP, op, "more than 2^28 queries of all heads, 65536 sequences or 2^22 "
+                                     "sequences of a KV head, or kv_row above 2^22");
   }
   if (!aligned16({q, k, v, o}) || !aligned4({offsets, lse})) {
     return refuse(VX_OP_EUNSUPP, op, "operands must be 16-byte aligned (offsets and lse 4-byte)");
