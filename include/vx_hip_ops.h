@@ -222,7 +222,7 @@ int64_t vx_nn_sample_workspace(int64_t rows, int64_t vocab);
  * whose table has a row a token. No counterpart in the reference.
  *
  * Arguments, devices and `workspace` as for many answers to one prompt above
- * (log probabilities use at most 160 KiB, the product 128 MiB). Outputs must not
+ * (log probabilities use at most 132 KiB, the product 128 MiB). Outputs must not
  * overlap inputs but where it is said. */
 
 /* The residual's addition and RMS norm of rows: s = x + residual, y = s *
@@ -258,7 +258,7 @@ int32_t vx_nn_quantize_i8_f32(const float *x, int8_t *q, float *q_scale,
  * `stride` elements apart (at least `rows`), bf16 or f32. The sum is exact; it
  * is rounded to f32, multiplied by x_scale, then by w_scale, in f32, and rounded
  * to y's type. cols a multiple of 16, at most 131056; x and w 16-byte aligned;
- * tokens and rows at most 2^24. */
+ * tokens and rows at most 2^24, and at most 2^22 tiles of 64 x 64 outputs. */
 int32_t vx_nn_gemm_i8_bf16(const int8_t *x, const float *x_scale,
                            const int8_t *w, const float *w_scale, uint16_t *y,
                            int64_t tokens, int64_t rows, int64_t cols,

@@ -1517,7 +1517,7 @@ int32_t vx_plugin_control(uint32_t opcode, void *payload) {
   }
   case VX_HIP_CTRL_OP_WORKSPACES: {
     /* payload -> int64_t[2]: workspaces held for the ops of a batch that
-     * shares a prompt (one per device and stream) and their bytes. */
+     * shares a prompt or is packed (one per device and stream) and their bytes. */
     int64_t *out = static_cast<int64_t *>(payload);
     if (!out) {
       return 0;

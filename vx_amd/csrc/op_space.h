@@ -1,7 +1,7 @@
 /*
  * op_space.h -- the workspaces that the library keeps for the ops of
- * ops_batch.cpp: one block per (device, stream), shared by the launches on
- * that stream, which run in order. A block grows as it is asked for (the old
+ * ops_batch.cpp and ops_packed.cpp: one block per (device, stream), shared by the
+ * launches on that stream, which run in order. A block grows as it is asked for (the old
  * one freed in the stream's order) and is freed, in that order, when the
  * calling thread's stream is set to another one; the default stream's stays.
  * A call that needs more than kOpSpaceKept has it for itself.

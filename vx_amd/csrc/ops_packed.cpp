@@ -56,7 +56,7 @@ int32_t gemm_extents(int64_t tokens, int64_t rows, int64_t cols, const char **wh
   }
   if (tokens > (int64_t(1) << 24) || rows > (int64_t(1) << 24) ||
       ((tokens + 63) / 64) * ((rows + 63) / 64) > (int64_t(1) << 22)) {
-    *why = "more than 2^24 tokens or rows, or 2^34 outputs";
+    *why = "more than 2^24 tokens or rows, or 2^22 tiles of 64 x 64 outputs";
     return VX_OP_EUNSUPP;
   }
   return VX_OP_OK;
