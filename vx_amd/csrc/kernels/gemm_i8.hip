@@ -7,6 +7,15 @@
  * have their columns together, so an MFMA operand is 16 bytes of a row: lane l
  * holds row l % 16, columns 16 (l / 16) .. + 15 of a stage of 64. The weights are
  * the first operand, so that a lane ends with 4 consecutive outputs of a token.
+ *
+ * Three kernels by the number of tokens (gemm_i8.h has the rules): one, few, and
+ * tiles. A tile's stage is 128 columns, since loads that take 64 of a row fetch
+ * each cache line in two turns (4096 x 11008 x 4096 266 us, whole lines and tiles
+ * of 256 x 256 159). That shape is 2.3 POP/s, of 8192^3 2.45-2.65: there MFMAs are
+ * busy 59% of the cycles, at a clock that the power limit holds at 1.75-1.93 GHz;
+ * no LDS conflicts. 777 x 6144 x 4096 takes 27: 224 tiles of 128 x 192, one round
+ * in which 32 CUs have none and a seventh of the last tile row is empty. 48 x 11008
+ * x 4096 takes 10-14, 172 workgroups that read 45 MB.
  */
 #include "../vx_hip_common.h"
 #include "../vx_packed_kernels.h"
@@ -102,7 +111,9 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t rs, uint32_t off)
 
 /* One token: a wave has 4 rows of w, whose bytes it reads 1 KiB at a time of
  * each, and adds up the products of its columns on v_dot4. With kSplit the four
- * waves of a workgroup have the same rows and take the pieces in turn. */
+ * waves of a workgroup have the same rows and take the pieces in turn. Bound by HBM:
+ * 32000 x 768 6.2 us (4.0 TB/s), 11008 x
+ * 4096 8.9 (5.1 TB/s). Of 2 rows 6.7 and 8.7, of 8 6.5 and 9.4. */
 constexpr int kRowsEach = 4;
 
 template <bool kF32, bool kSplit>
@@ -180,12 +191,15 @@ __global__ __launch_bounds__(256) void gemm_i8_row(GemmI8Args a) {
 
 /* Few tokens: a workgroup has 16 rows of w and all tokens, its waves take lines
  * of 128 columns in turn, kAhead at once, from memory into registers, and meet in
- * LDS. */
+ * LDS. 8 waves: 16 tokens x 32000 x 768 8.3 us, and 8.8 in 4, 12.7 in 16. 16 x 11008
+ * x 4096 14.0, 3.2 TB/s: bound by the loads in flight, a wave a line of each row. */
+constexpr int kFewWaves = 8;
 constexpr uint32_t kPast = 0x7ffffff0u; /* an offset past any buffer's end: reads zeros */
 using i8::kLine;
 
-template <bool kF32, int kTT, int kWaves, int kAhead>
-__global__ __launch_bounds__(64 * kWaves) void gemm_i8_few(GemmI8Args a) {
+template <bool kF32, int kTT, int kAhead>
+__global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few(GemmI8Args a) {
+  constexpr int kWaves = kFewWaves;
   __shared__ i32x4 part[kWaves][kTT][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -540,21 +554,18 @@ template <bool kF32> void row(const GemmI8Args &a, hipStream_t stream) {
   }
 }
 
-template <bool kF32, int kTT, int kWaves, int kAhead>
-void few_ahead(const GemmI8Args &a, hipStream_t stream) {
-  hipLaunchKernelGGL((gemm_i8_few<kF32, kTT, kWaves, kAhead>), dim3((unsigned)((a.rows + 15) / 16)),
-                     dim3(64 * kWaves), 0, stream, a);
+template <bool kF32, int kTT, int kAhead> void few_ahead(const GemmI8Args &a, hipStream_t stream) {
+  hipLaunchKernelGGL((gemm_i8_few<kF32, kTT, kAhead>), dim3((unsigned)((a.rows + 15) / 16)),
+                     dim3(64 * kFewWaves), 0, stream, a);
 }
+/* A wave's lines at once, 1 and 4: 16 tokens x 32000 x 1024 10.1 us and 16.5, 4096 x
+ * 4096 7.2 and 6.7, 11008 x 4096 14.9 and 14.0; 24 x 4096 x 4096 7.7 and 8.0, 16000 x
+ * 1024 7.7 and 11.9. */
 template <bool kF32, int kTT> void few(const GemmI8Args &a, hipStream_t stream) {
-  const int lines = (a.cols + kLine - 1) / kLine;
-  if (lines <= 4) {
-    few_ahead<kF32, kTT, 4, 1>(a, stream);
-  } else if (lines <= 8) {
-    few_ahead<kF32, kTT, 8, 1>(a, stream);
-  } else if (kTT > 1 || lines <= 16) {
-    few_ahead<kF32, kTT, 8, 2>(a, stream);
+  if (kTT == 1 && a.cols > kFewWaves * kLine) {
+    few_ahead<kF32, kTT, kTT == 1 ? 4 : 1>(a, stream);
   } else {
-    few_ahead<kF32, kTT, 8, kTT == 1 ? 4 : 2>(a, stream);
+    few_ahead<kF32, kTT, 1>(a, stream);
   }
 }
 
