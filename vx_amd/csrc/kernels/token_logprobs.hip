@@ -39,6 +39,7 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kSlack = 8.0f;
+constexpr float kFar = -1000.0f; /* e^kFar is 0 */
 constexpr int kMostTop = 64;
 
 /* Rises with l; 0 for -inf and NaN, which are no alternatives. */
@@ -61,9 +62,11 @@ __device__ __forceinline__ int index_of(u64 key) { return (int)~(u32)key; }
 struct Sums {
   float m, s, e;
 };
-/* Against `top`, which is no lower than any logit in them. */
+/* Against `top`, which is no lower than any logit in them. e^-1000 is 0 in f32, and s
+ * times it too: the distance itself may be past the largest f32 (a part in which all
+ * is masked by the type's lowest value), and 0 times infinity a NaN. */
 __device__ __forceinline__ Sums against(Sums v, float top) {
-  const float d = v.m - top;
+  const float d = fmaxf(v.m - top, kFar);
   const float f = __builtin_amdgcn_exp2f(d * kLog2e);
   return v.s > 0.0f ? Sums{top, v.s * f, f * (v.e + v.s * d)} : Sums{top, 0.0f, 0.0f};
 }
@@ -113,6 +116,19 @@ struct Row {
   float top, log_sum, entropy;
   bool inf; /* a logit is +inf: those alone count, equally */
 };
+/* From the sums against `top`, or how many are +inf. Rounding may leave an entropy
+ * below 0; a NaN stays one. */
+__device__ __forceinline__ Row row_of(float top, float s, float e, int infs) {
+  if (top == INFINITY) {
+    const float n = logf((float)infs);
+    return Row{top, n, n, true};
+  }
+  if (!(top > -INFINITY)) {
+    return Row{top, 0.0f, 0.0f, false};
+  }
+  const float log_sum = logf(s), entropy = log_sum - e / s;
+  return Row{top, log_sum, entropy < 0.0f ? 0.0f : entropy, false};
+}
 __device__ __forceinline__ float logprob_of(const Row &r, float x) {
   if (r.inf) {
     return x == INFINITY ? -r.log_sum : -INFINITY;
@@ -225,7 +241,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(LogprobArgs a, Logprob
 #pragma unroll
     for (int e = 0; e < kN; ++e) {
       /* -inf and NaN weigh nothing */
-      const float d = fmaxf(v[e] - acc.m, -1000.0f);
+      const float d = fmaxf(v[e] - acc.m, kFar);
       const float w = __builtin_amdgcn_exp2f(d * kLog2e);
       acc.s += w;
       acc.e = __builtin_fmaf(w, d, acc.e);
@@ -302,7 +318,7 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(LogprobArgs a, Logprob
     e += sh.b[i];
     infs += sh.n[i];
   }
-  Row row{top, 0.0f, 0.0f, inf};
+  const Row row = row_of(top, s, e, infs);
   if constexpr (kSliced) {
     if (t == 0) {
       Part &p = parts[blockIdx.x];
@@ -312,8 +328,6 @@ __global__ __launch_bounds__(kThreads) void logprobs_rows(LogprobArgs a, Logprob
       p.infs = infs;
     }
   } else {
-    row.log_sum = inf ? logf((float)infs) : none ? 0.0f : logf(s);
-    row.entropy = inf ? row.log_sum : none ? 0.0f : fmaxf(row.log_sum - e / s, 0.0f);
     write_given<kThreads>(a, r, row);
     if (a.entropy && t == 0) {
       a.entropy[r] = row.entropy;
@@ -474,9 +488,7 @@ __global__ __launch_bounds__(kMergeThreads) void logprobs_merge(LogprobArgs a, L
   const bool none = !(top > -INFINITY), inf = top == INFINITY;
   const Sums v = has && !none && !inf ? against(own, top) : Sums{0.0f, 0.0f, 0.0f};
   const float s = wave_sum(v.s), e = wave_sum(v.e);
-  Row row{top, 0.0f, 0.0f, inf};
-  row.log_sum = inf ? logf((float)infs) : none ? 0.0f : logf(s);
-  row.entropy = inf ? row.log_sum : none ? 0.0f : fmaxf(row.log_sum - e / s, 0.0f);
+  const Row row = row_of(top, s, e, infs);
   write_given<kMergeThreads>(a, r, row);
   if (a.entropy && threadIdx.x == 0) {
     a.entropy[r] = row.entropy;
