@@ -198,7 +198,7 @@ __global__ __launch_bounds__(kThreads, 2) void flash_packed(KernelArgs p) {
   constexpr int kDSteps = kD / 16;
   constexpr int kDTiles = kD / 32;
   constexpr int kRowBytes = kD * 2;
-  __shared__ __attribute__((aligned(16))) char lds[4 * kBK * kD * 2];
+  __shared__ __align__(kRowBytes) char lds[4 * kBK * kD * 2]; /* addresses of a row are XORed */
 
   /* Workgroup i runs on XCD i % 8: where the KV heads are a multiple of 8, each
    * XCD has its own, whose keys its L2 then holds alone. */
