@@ -222,8 +222,8 @@ int64_t vx_nn_sample_workspace(int64_t rows, int64_t vocab);
  * whose table has a row a token. No counterpart in the reference.
  *
  * Arguments, devices and `workspace` as for many answers to one prompt above
- * (log probabilities use at most 132 KiB, the product 128 MiB). Outputs must not
- * overlap inputs but where it is said. */
+ * (log probabilities use at most 132 KiB, the product 64 KiB a CU, 16 MiB on 256).
+ * Outputs must not overlap inputs but where it is said. */
 
 /* The residual's addition and RMS norm of rows: s = x + residual, y = s *
  * (mean s^2 + eps)^-1/2 * weight, the mean in 64 bits.

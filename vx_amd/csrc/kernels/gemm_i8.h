@@ -42,13 +42,13 @@ constexpr Tile kTile[] = {{64, 64, 2, 2.1, 0.42, 0.25},   {128, 128, 1, 2.9, 0.6
 constexpr int kTiles = sizeof(kTile) / sizeof(kTile[0]);
 constexpr int kSplitTiles = 2; /* the first of them, which may be split */
 constexpr int kMaxSplits = 16;
-constexpr int64_t kMaxBytes = (int64_t)128 << 20;
 
 inline int64_t count(const Tile &t, int64_t tokens, int64_t rows) {
   return ((tokens + t.bm - 1) / t.bm) * ((rows + t.bn - 1) / t.bn);
 }
 
-/* Splits leave 4 bytes a sum in a workspace, which a second launch reads. */
+/* Splits leave 4 bytes a sum in a workspace, which a second launch reads. They are
+ * no more than fit the CUs at once, 64 KiB a CU: one tile of 128x128 or two of 64x64. */
 inline int64_t ws_bytes(const Tile &t, int64_t tokens, int64_t rows, int splits) {
   return splits > 1 ? count(t, tokens, rows) * splits * t.bm * t.bn * 4 : 0;
 }
@@ -87,8 +87,7 @@ inline GemmI8Plan gemm_i8_plan(int64_t tokens, int64_t rows, int64_t cols, int c
     const i8::Tile &t = i8::kTile[i];
     const int64_t units = i8::count(t, tokens, rows), lines = (cols + i8::kLine - 1) / i8::kLine;
     for (int s = 1; s <= (may_split && i < i8::kSplitTiles ? i8::kMaxSplits : 1); ++s) {
-      if (s > 1 && (units * s > (int64_t)t.per_cu * cus || lines < 4 * s ||
-                    i8::ws_bytes(t, tokens, rows, s) > i8::kMaxBytes)) {
+      if (s > 1 && (units * s > (int64_t)t.per_cu * cus || lines < 4 * s)) {
         break;
       }
       const double v = i8::us(t, tokens, rows, cols, s, cus);
