@@ -335,8 +335,9 @@ __device__ __forceinline__ void store_blocks(const GemmI8Args &a, const i32x4 (&
  * buffer-to-LDS loads. Planes are [rows][8 chunks of 16 columns], chunk c of a row
  * at place c ^ (row % 8), so that reads of 16 rows at one chunk meet every bank.
  * With kMid a slot's plane of w is filled again from the middle of its stage on,
- * when all of it is in registers. */
-template <bool kF32, int kBM, int kBN, int kWM, int kWN, int kNS, bool kMid, int kPerCu>
+ * when all of it is in registers. With kSplits several workgroups may divide a tile's
+ * stages, whose sums gemm_i8_join adds up. */
+template <bool kF32, int kBM, int kBN, int kWM, int kWN, int kNS, bool kMid, int kPerCu, bool kSplits>
 __global__ __launch_bounds__(64 * kWM * kWN, kPerCu * kWM * kWN / 4) void gemm_i8_tiles(
     GemmI8Args a, int tiles_m, int tiles_n, int splits, i32x4 *__restrict__ parts) {
   constexpr int kThreads = 64 * kWM * kWN;
@@ -353,15 +354,15 @@ __global__ __launch_bounds__(64 * kWM * kWN, kPerCu * kWM * kWN / 4) void gemm_i
   const int g = lane >> 4;
   const int wm = wave / kWN, wn = wave % kWN;
   const int tiles = tiles_m * tiles_n;
-  const int split = (int)blockIdx.x / tiles;
+  const int split = kSplits ? (int)blockIdx.x / tiles : 0;
   const int id = (int)blockIdx.x - split * tiles;
   const pp::Tile tile = pp::tile_of(id, tiles, tiles_m, tiles_n);
   const int64_t m0 = (int64_t)tile.tm * kBM;
   const int64_t n0 = (int64_t)tile.tn * kBN;
   /* this workgroup's stages */
   const int all = (a.cols + kLine - 1) / kLine;
-  const int first = (int)((int64_t)all * split / splits);
-  const int stages = (int)((int64_t)all * (split + 1) / splits) - first;
+  const int first = kSplits ? (int)((int64_t)all * split / splits) : 0;
+  const int stages = kSplits ? (int)((int64_t)all * (split + 1) / splits) - first : all;
   const int cols = a.cols;
 
   /* Load p of a wave fills rows (wave * kLA + p) * 8 + lane / 8 of a plane; its
@@ -498,7 +499,7 @@ __global__ __launch_bounds__(64 * kWM * kWN, kPerCu * kWM * kWN / 4) void gemm_i
     slot = after;
   }
 
-  if (splits > 1) {
+  if (kSplits && splits > 1) {
     i32x4 *to = parts + ((int64_t)blockIdx.x * kTM * kTN) * kThreads + threadIdx.x;
 #pragma unroll
     for (int i = 0; i < kTM; ++i) {
@@ -569,16 +570,18 @@ template <bool kF32, int kTT> void few(const GemmI8Args &a, hipStream_t stream) 
   }
 }
 
-template <bool kF32, int kBM, int kBN, int kWM, int kWN, int kNS, bool kMid, int kPerCu>
+template <bool kF32, int kBM, int kBN, int kWM, int kWN, int kNS, bool kMid, int kPerCu, bool kSplits>
 void tiles(const GemmI8Args &a, int splits, char *ws, hipStream_t stream) {
   const int tm = (int)((a.tokens + kBM - 1) / kBM), tn = (int)((a.rows + kBN - 1) / kBN);
-  hipLaunchKernelGGL((gemm_i8_tiles<kF32, kBM, kBN, kWM, kWN, kNS, kMid, kPerCu>),
+  hipLaunchKernelGGL((gemm_i8_tiles<kF32, kBM, kBN, kWM, kWN, kNS, kMid, kPerCu, kSplits>),
                      dim3((unsigned)(tm * tn * splits)), dim3(64 * kWM * kWN), 0, stream, a, tm, tn,
                      splits, reinterpret_cast<i32x4 *>(ws));
-  if (splits > 1) {
-    const int64_t all = (int64_t)tm * tn * (kBM * kBN / 4);
-    hipLaunchKernelGGL((gemm_i8_join<kF32, kBM, kBN, kWM, kWN>), dim3((unsigned)((all + 255) / 256)),
-                       dim3(256), 0, stream, a, tm, tn, splits, reinterpret_cast<const i32x4 *>(ws));
+  if constexpr (kSplits) {
+    if (splits > 1) {
+      const int64_t all = (int64_t)tm * tn * (kBM * kBN / 4);
+      hipLaunchKernelGGL((gemm_i8_join<kF32, kBM, kBN, kWM, kWN>), dim3((unsigned)((all + 255) / 256)),
+                         dim3(256), 0, stream, a, tm, tn, splits, reinterpret_cast<const i32x4 *>(ws));
+    }
   }
 }
 
@@ -588,18 +591,18 @@ void launch(const GemmI8Args &a, const GemmI8Plan &p, char *ws, hipStream_t stre
     row<kF32>(a, stream);
   } else if (p.kind == GemmI8Plan::kFew) {
     a.tokens <= 16 ? few<kF32, 1>(a, stream) : few<kF32, 2>(a, stream);
-  } else if (p.tile == 0) {
-    tiles<kF32, 64, 64, 2, 2, 4, false, 2>(a, p.splits, ws, stream);
+  } else if (p.tile == 0) { /* i8::kSplitTiles of them may be split */
+    tiles<kF32, 64, 64, 2, 2, 4, false, 2, true>(a, p.splits, ws, stream);
   } else if (p.tile == 1) {
-    tiles<kF32, 128, 128, 4, 2, 4, false, 1>(a, p.splits, ws, stream);
+    tiles<kF32, 128, 128, 4, 2, 4, false, 1, true>(a, p.splits, ws, stream);
   } else if (p.tile == 2) {
-    tiles<kF32, 128, 128, 4, 2, 2, true, 2>(a, 1, nullptr, stream);
+    tiles<kF32, 128, 128, 4, 2, 2, true, 2, false>(a, 1, nullptr, stream);
   } else if (p.tile == 3) {
-    tiles<kF32, 128, 192, 4, 2, 3, false, 1>(a, 1, nullptr, stream);
+    tiles<kF32, 128, 192, 4, 2, 3, false, 1, false>(a, 1, nullptr, stream);
   } else if (p.tile == 4) {
-    tiles<kF32, 256, 128, 4, 2, 3, false, 1>(a, 1, nullptr, stream);
+    tiles<kF32, 256, 128, 4, 2, 3, false, 1, false>(a, 1, nullptr, stream);
   } else {
-    tiles<kF32, 256, 256, 4, 2, 2, true, 1>(a, 1, nullptr, stream);
+    tiles<kF32, 256, 256, 4, 2, 2, true, 1, false>(a, 1, nullptr, stream);
   }
 }
 
