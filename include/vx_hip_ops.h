@@ -286,9 +286,11 @@ int64_t vx_nn_gemm_i8_workspace(int64_t tokens, int64_t rows, int64_t cols);
  * outside the tensors is read or written, but which outputs are is not said.
  * lse: [heads, total] f32 (may be NULL), natural logarithm.
  * With `causal`, a query sees its sequence's keys up to its own row; else all.
- * Numerics, `scale` and what hidden keys may hold as in
- * vx_nn_flash_attention_shared_bf16. head_dim 64 or 128; strides multiples of 8,
- * at least head_dim; kv_row at most 2^22; pointers 16-byte aligned; at most
+ * Numerics (the weights' rounding to bf16 among them: o is off by 1.8e-3 to
+ * 2.0e-3 of its size, where the rounding of o itself makes 1.5e-3 to 1.6e-3),
+ * `scale` and what hidden keys may hold as in
+ * vx_nn_flash_attention_shared_bf16. head_dim 64 or 128; strides multiples of
+ * 8, at least head_dim; kv_row at most 2^22; pointers 16-byte aligned; at most
  * 65536 sequences, 2^22 sequences * kv_heads and 2^28 queries of all heads. */
 int32_t vx_nn_flash_attention_packed_bf16(
     const uint16_t *q, const uint16_t *k, const uint16_t *v,

@@ -18,7 +18,8 @@
  * divide the keys and meet in LDS.
  * The weights are rounded to bf16, off by at most 2^-8 each, because the second
  * product's operands are bf16 (f32 ones multiply at a sixteenth of the rate);
- * maxima and sums stay in f32, the sums over unrounded weights.
+ * maxima and sums stay in f32, the sums over unrounded weights. It takes o from
+ * 1.5e-3-1.6e-3 of its 2-norm, its own rounding, to 1.8e-3-2.0e-3.
  *
  * Where V holds infinities or NaNs, a key hidden from a query reaches it all the
  * same (0 x inf is NaN): a workgroup whose outputs are not all finite goes over its
@@ -27,13 +28,14 @@
  * With that beside the loop instead of in it, the loop's registers stay in place:
  * 8192 and 91 tokens, 32 heads on 8, 627 -> 552 us.
  *
- * 550 us there, 1.0 PFLOP/s, is bound by the CU's parts taking turns: a turn of two
- * workgroups (2.0 us) needs 0.86 of MFMAs, 0.95 of the softmax's VALU and 1.2 of
- * LDS. 64 sequences of 1 to 1024 tokens take 90: a workgroup of 4.6 turns spends 2
- * us to find its tile, 3 until its first keys are there, and 2.6 after the last.
- * Workgroups that go from tile to tile and load the next one's keys in between
- * needed registers that the loop's values were then moved and spilled for: 116 us,
- * and 590 for the long one.
+ * 537-550 us there, 1.0 PFLOP/s (without a mask 1136, 0.97), is bound by the CU's
+ * parts taking turns: a turn of two workgroups (2.0 us) needs 0.86 of MFMAs, 0.95
+ * of the softmax's VALU and 1.2 of LDS. 64 sequences of 1 to 1024 tokens take 90
+ * (135 without a mask): a workgroup of 4.6 turns spends 2 us to find its tile, 3
+ * until its first keys are there, and 2.6 after the last. Workgroups that go from
+ * tile to tile and load the next one's keys in between needed registers that the
+ * loop's values were then moved and spilled for: 116 us, and 590 for the long
+ * one.
  */
 #include "../vx_hip_common.h"
 #include "../vx_packed_kernels.h"

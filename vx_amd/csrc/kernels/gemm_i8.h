@@ -77,8 +77,13 @@ inline GemmI8Plan gemm_i8_plan(int64_t tokens, int64_t rows, int64_t cols, int c
     return p;
   }
   if (tokens <= 16 || (tokens <= 32 && rows * cols <= (int64_t(1) << 24))) {
-    /* 24 x 4096 x 4096 8.0 us, and 11 by tiles; 32 x 11008 x 4096 21 and 14, 32 x
-     * 32000 x 768 12.8 and 8.2; 16 x 11008 x 4096 14 and 13.3 */
+    /* In us, by this kernel and by tiles, weights from HBM: 2 x 11008 x 4096 10.9 and
+     * 13.2, 16 x 4096 x 4096 6.7 and 9.2, 24 x 4096 x 4096 7.6 and 9.3, 32 x 4096 x 4096
+     * 8.3 and 9.5, 24 x 768 x 2048 5.0 and 7.4; past the border 32 x 11008 x 4096 21 and
+     * 13.7, 32 x 32000 x 768 12.8 and 7.7. It is drawn by tokens and weights alone, and
+     * near it gives some away where rows are many: 16 x 11008 x 4096 14.0 and 13.4, 16 x
+     * 32000 x 768 8.3 and 7.5, 16 x 32000 x 1024 10.2 and 8.8, 24 x 16000 x 1024 7.9 and
+     * 6.2. */
     p.kind = GemmI8Plan::kFew;
     return p;
   }

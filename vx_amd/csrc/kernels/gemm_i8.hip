@@ -11,11 +11,12 @@
  * Three kernels by the number of tokens (gemm_i8.h has the rules): one, few, and
  * tiles. A tile's stage is 128 columns, since loads that take 64 of a row fetch
  * each cache line in two turns (4096 x 11008 x 4096 266 us, whole lines and tiles
- * of 256 x 256 159). That shape is 2.3 POP/s, of 8192^3 2.45-2.65: there MFMAs are
- * busy 59% of the cycles, at a clock that the power limit holds at 1.75-1.93 GHz;
- * no LDS conflicts. 777 x 6144 x 4096 takes 27: 224 tiles of 128 x 192, one round
- * in which 32 CUs have none and a seventh of the last tile row is empty. 48 x 11008
- * x 4096 takes 10-14, 172 workgroups that read 45 MB.
+ * of 256 x 256 163-168). That shape is 2.2-2.3 POP/s, of 8192^3 2.4-2.7: there MFMAs
+ * are busy 59% of the cycles, at a clock that the power limit holds at 1.75-1.93 GHz;
+ * no LDS conflicts. 777 x 6144 x 4096 takes 27: 224 tiles of 128 x 192, one round in
+ * which 32 CUs have none and a seventh of the last tile row is empty. 48 x 11008 x
+ * 4096, 172 workgroups that read 45 MB, takes 10.4 where the last-level cache holds
+ * the weights and 13.9 from HBM.
  */
 #include "../vx_hip_common.h"
 #include "../vx_packed_kernels.h"
@@ -112,8 +113,8 @@ __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t rs, uint32_t off)
 /* One token: a wave has 4 rows of w, whose bytes it reads 1 KiB at a time of
  * each, and adds up the products of its columns on v_dot4. With kSplit the four
  * waves of a workgroup have the same rows and take the pieces in turn. Bound by HBM:
- * 32000 x 768 6.2 us (4.0 TB/s), 11008 x
- * 4096 8.9 (5.1 TB/s). Of 2 rows 6.7 and 8.7, of 8 6.5 and 9.4. */
+ * 32000 x 768 6.2 us (4.0 TB/s), 11008 x 4096 8.9 (5.1 TB/s), and where the last-level
+ * cache holds the weights 4.9 and 7.1. Of 2 rows 6.7 and 8.7, of 8 6.5 and 9.4. */
 constexpr int kRowsEach = 4;
 
 template <bool kF32, bool kSplit>
@@ -192,7 +193,7 @@ __global__ __launch_bounds__(256) void gemm_i8_row(GemmI8Args a) {
 /* Few tokens: a workgroup has 16 rows of w and all tokens, its waves take lines
  * of 128 columns in turn, kAhead at once, from memory into registers, and meet in
  * LDS. 8 waves: 16 tokens x 32000 x 768 8.3 us, and 8.8 in 4, 12.7 in 16. 16 x 11008
- * x 4096 14.0, 3.2 TB/s: bound by the loads in flight, a wave a line of each row. */
+ * x 4096 14.0, 3.2 TB/s of weights, and as many bytes of x through the caches. */
 constexpr int kFewWaves = 8;
 constexpr uint32_t kPast = 0x7ffffff0u; /* an offset past any buffer's end: reads zeros */
 using i8::kLine;
@@ -266,7 +267,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void gemm_i8_few(GemmI8Args a) {
 /* A wave's kTM x kTN blocks of outputs from token t0 and row r0 on, 16 tokens at
  * a time through LDS (`mine`, the wave's own), so that a store has whole lines of a
  * token's row: 16 lanes with 4 rows each, as the products leave them, would store
- * 32 bytes of each (4096 x 32000 x 768 in bf16 208 us, and 144 this way). */
+ * 32 bytes of each (4096 x 32000 x 768 in bf16 208 us, and 144-149 this way: six
+ * stages a tile, and one workgroup a CU, whose stores nothing overlaps). */
 template <bool kF32, int kTM, int kTN>
 __device__ __forceinline__ void store_blocks(const GemmI8Args &a, const i32x4 (&acc)[kTM][kTN],
                                              int64_t t0, int64_t r0, char *mine) {

@@ -18,9 +18,9 @@
  * likeliest in a workspace, logprobs_merge adds them up.
  *
  * 512 x 131071 bf16 with entropy and 20 alternatives 36 us, of which 31 without
- * alternatives (4.35 TB/s: the row's reading bounds it), 2048 x 32000 f32 44 (5.9
- * TB/s) and 55 with 5 alternatives. 1 x 32000 9.1: 5.8 for the sums, of which half
- * the launch, and 3.3 for the alternatives, a chain of barriers and two loads.
+ * alternatives (4.3 TB/s: the row's reading bounds it), 2048 x 32000 f32 44-47 (5.6-5.9
+ * TB/s) and 55 with 5 alternatives. 1 x 32000 9.2: two launches, 6.5 for its two slices,
+ * a chain of barriers and dependent loads, and 2.6 for the merge.
  */
 #include "../vx_hip_common.h"
 #include "../vx_packed_kernels.h"
@@ -538,7 +538,8 @@ void launch(const LogprobArgs &a, const LogprobPlan &plan, Part *parts, hipStrea
  * each. In us, undivided and in 2, 4, 8 and 16: 1 x 131072 with 5 alternatives 18,
  * 16.2, 11.8, 10.3 and 10.2; 1 x 50257 10.8, 10.8, 9.7, 9.6 and 10.4; 16 x 131072
  * with 20 17.7, 15.3, 13.2, 13.3 and 19.9; 64 rows 20.2, 19.4, 15.7, 17.2 and 25;
- * 128 rows 22.2, 21.5, 20.7, 22.9 and 32. */
+ * 128 rows 22.2, 21.5, 20.7, 22.9 and 32 (more workgroups than CUs gain 4% there, and
+ * nothing with 64 rows). */
 LogprobPlan logprobs_plan(int64_t rows, int64_t vocab, int64_t n_top, bool may_split) {
   LogprobPlan p{1, (int)vocab, 0};
   const int64_t want = std::min<int64_t>(
